@@ -1,0 +1,422 @@
+"""The row operators that stand beside the fold: layer norm over the folded partials of the ranks, its gradient with the
+reduction of the weight's and bias's gradients, and activation checkpoints in 8 bits with their use in the backward pass.
+
+Each case is one pass of an operator (or of the two that belong together in a training step), computed in plain torch
+operations in 32 bits, or by the library's persistent handles where `own` is true.
+
+Definitions (rows r, columns c, n columns, blocks of 128 columns):
+  fold        x = round((((src0 + src1) + ...) + residual)), added in 32 bits, rounded once to the tensors' type
+  layer norm  mean = sum_c x / n, rstd = 1 / sqrt(sum_c (x - mean)^2 / n + eps), y = (x - mean) * rstd * w + b
+  gradient    g = dy0 + dy1 + ..., xh = (x - mean) * rstd, dw = sum_r g * xh, db = sum_r g,
+              dx = rstd * (g * w - sum_c(g * w) / n - xh * sum_c(g * w * xh) / n) + dsum
+  checkpoint  a = max(max_block |x|, 2^-100), q = rint(x * (127 / a)) in 8 bits, scale = a * (1 / 127), restored q * scale
+              (127 / a, 1 / 127 and both products rounded to 32 bits)
+  activation  h = act(a), or act(a) * b with a gate; dh is taken back through the restored a and b
+"""
+import functools
+import math
+
+import torch
+
+own = False
+
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+BLOCK = 128
+EPS = 1e-5
+TINY = 2.0 ** -100
+INV127 = float(torch.tensor(1.0 / 127.0, dtype=torch.float32))
+
+
+def listed():
+    return [
+        # one token of a decode step: the partial rows of 8 ranks folded onto the residual stream, then its norm
+        {"name": "norm_token", "op": "norm", "rows": 1, "cols": 4096, "type": "bf16", "nsrc": 8, "residual": True, "w32": False, "pad": 0},
+        # a prefill's rows after one sum, with the residual
+        {"name": "norm_prefill", "op": "norm", "rows": 4096, "cols": 8192, "type": "bf16", "nsrc": 1, "residual": True, "w32": False, "pad": 0},
+        # odd sizes, rows that start at any element, 4 ranks' partials in 32 bits
+        {"name": "norm_odd", "op": "norm", "rows": 1021, "cols": 5003, "type": "fp32", "nsrc": 4, "residual": False, "w32": True, "pad": 3},
+        # a training batch's backward pass with the gradient of the residual stream added, 32-bit weight gradients
+        {"name": "grad_batch", "op": "grad", "rows": 16384, "cols": 4096, "type": "bf16", "nsrc": 1, "residual": True, "w32": True, "pad": 0},
+        # a short sequence's backward pass, two ranks' partial gradients folded
+        {"name": "grad_short", "op": "grad", "rows": 29, "cols": 1024, "type": "fp16", "nsrc": 2, "residual": False, "w32": False, "pad": 0},
+        # a training step's norm, forward and backward, its input kept in 8 bits between the two
+        {"name": "step8_batch", "op": "step8", "rows": 8192, "cols": 5120, "type": "bf16", "nsrc": 1, "residual": True, "w32": True, "pad": 0},
+        # the same in 32 bits at odd sizes
+        {"name": "step8_odd", "op": "step8", "rows": 509, "cols": 1111, "type": "fp32", "nsrc": 1, "residual": False, "w32": True, "pad": 0},
+        # a layer's activations written to 8 bits and restored
+        {"name": "ckpt8_layer", "op": "ckpt8", "rows": 8192, "cols": 16384, "type": "bf16", "pad": 0},
+        # the same for a few rows, where latency counts
+        {"name": "ckpt8_few", "op": "ckpt8", "rows": 16, "cols": 2048, "type": "fp16", "pad": 0},
+        # a gated feed-forward layer's activation, forward and backward, a and b halves of one product's rows
+        {"name": "act8_gated", "op": "act8", "rows": 8192, "cols": 12288, "type": "bf16", "act": "silu", "gate": True, "pad": 0},
+        # an ungated one at an odd width
+        {"name": "act8_odd", "op": "act8", "rows": 777, "cols": 4099, "type": "fp16", "act": "gelu", "gate": False, "pad": 1},
+        # a few tokens in 32 bits
+        {"name": "act8_few", "op": "act8", "rows": 4, "cols": 8192, "type": "fp32", "act": "gelu_tanh", "gate": True, "pad": 0},
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["norm", "norm", "grad", "step8", "ckpt8", "act8"])
+    case = {"op": op, "rows": _log(rng, 1, 16384), "cols": _log(rng, 64, 16384), "type": rng.choice(["bf16", "bf16", "fp16", "fp32"]),
+            "pad": rng.choice([0, 0, 8, 3])}
+    if rng.random() < 0.5:
+        case["cols"] = max(64, case["cols"] // 64 * 64)
+    if op in ("norm", "grad", "step8"):
+        case["nsrc"] = 1 if op == "step8" else rng.choice([1, 1, 2, 4, 8])
+        case["residual"] = rng.random() < 0.5
+        case["w32"] = rng.random() < 0.5
+    if op == "act8":
+        case["act"] = rng.choice(["silu", "gelu", "gelu_tanh"])
+        case["gate"] = rng.random() < 0.6
+    top = max(work(c)["bytes"] for c in listed() if c["op"] == op)
+    case["rows"] = max(1, min(case["rows"], int(case["rows"] * top / work(case)["bytes"])))
+    return case
+
+
+def _esize(case):
+    return 4 if case["type"] == "fp32" else 2
+
+
+def work(case):
+    n, c, e = case["rows"] * case["cols"], case["cols"], _esize(case)
+    saved = n + 4 * case["rows"] * -(-c // BLOCK)  # a checkpoint's bytes
+    op = case["op"]
+    if op == "ckpt8":
+        return {"bytes": 2 * n * e + 2 * saved, "flops": 5 * n}
+    if op == "act8":
+        k = 2 if case["gate"] else 1  # in and out: a, b, h, dh, da, db
+        return {"bytes": n * e * (2 * k + 2) + 2 * k * saved, "flops": 30 * n}
+    w = 4 if case["w32"] else e
+    res = 1 if case["residual"] else 0
+    summed = 1 if case["residual"] or case["nsrc"] > 1 else 0
+    if op == "norm":
+        return {"bytes": n * e * (case["nsrc"] + res + summed + 1) + 8 * case["rows"] + 2 * c * w, "flops": (case["nsrc"] + 8) * n}
+    if op == "grad":
+        return {"bytes": n * e * (case["nsrc"] + res + 2) + 8 * case["rows"] + 3 * c * w, "flops": (case["nsrc"] + 14) * n}
+    return {"bytes": n * e * (1 + res + summed + 1 + 1 + res + 1) + 2 * saved + 16 * case["rows"] + 5 * c * w, "flops": 30 * n}
+
+
+# ---- inputs ----
+
+def _rand(gen, case, scale=1.0, cols=None):
+    """[rows, cols] of the case's type, its rows `pad` elements apart."""
+    rows, cols = case["rows"], cols or case["cols"]
+    t = torch.randn(rows, cols + case["pad"], device="cuda", generator=gen)
+    return t.mul_(scale).to(TYPES[case["type"]])[:, :cols]
+
+
+def _inputs(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    rows, cols, dt = case["rows"], case["cols"], TYPES[case["type"]]
+    op, i = case["op"], {}
+    if op == "ckpt8":
+        i["x"] = _rand(gen, case)
+        i["x"][:, :: 97] *= 16  # a few columns far larger than the rest, as activations have
+        return i
+    if op == "act8":
+        k = 2 if case["gate"] else 1
+        ab = _rand(gen, case, 1.5, k * cols)  # one product's rows: a, then b
+        i["a"] = ab[:, :cols]
+        if case["gate"]:
+            i["b"] = ab[:, cols:]
+        i["dh"] = _rand(gen, case, 0.25)
+        return i
+    wt = torch.float32 if case["w32"] else dt
+    i["w"] = (1 + 0.2 * torch.randn(cols, device="cuda", generator=gen)).to(wt)
+    if op in ("norm", "step8"):
+        i["b"] = (0.1 * torch.randn(cols, device="cuda", generator=gen)).to(wt)
+        i["src"] = [_rand(gen, case, case["nsrc"] ** -0.5) for _ in range(case["nsrc"])]
+        if case["residual"]:
+            i["res"] = _rand(gen, case, 2.0)
+            i["res"][:, :: 211] *= 16
+    if op in ("grad", "step8"):
+        i["dy"] = [_rand(gen, case, 0.3) for _ in range(case["nsrc"])]
+        if case["residual"]:
+            i["dsum"] = _rand(gen, case, 0.3)
+    if op == "grad":
+        i["x"] = _rand(gen, case, 2.0)
+        x = i["x"].double()
+        mean = x.mean(1, keepdim=True)
+        i["mean"] = mean[:, 0].float()
+        i["rstd"] = ((x - mean).square().mean(1) + EPS).rsqrt().float()
+    return i
+
+
+class _Handles:
+    """The persistent handles of a state, released with it."""
+
+    def __init__(self, *handles):
+        import ext_mpi_collectives_amd as emac
+        self.start, self.done, self.all = emac.start, emac.done, handles
+        for h in handles:
+            emac.set_stream(h, torch.cuda.current_stream().cuda_stream)
+
+    def __del__(self):
+        for h in self.all:
+            self.done(h)
+
+
+def _empty(case, cols=None, dt=None):
+    return torch.empty(case["rows"], cols or case["cols"], device="cuda", dtype=dt or TYPES[case["type"]])
+
+
+def _saved(case):
+    """A checkpoint's bytes, rows 16-byte aligned, and its scales."""
+    c = case["cols"]
+    return _empty(case, -(-c // 16) * 16, torch.int8), _empty(case, -(-c // BLOCK), torch.float32)
+
+
+def prepare(case, seed):
+    s = {"case": case, "in": _inputs(case, seed)}
+    if own:
+        s["out"], s["handles"], s["kept"] = _handles(case, s["in"])
+    return s
+
+
+def _handles(case, i):
+    """The outputs' buffers, the handles on them, and what else they point to."""
+    import ext_mpi_collectives_amd as emac
+    op, rows, cols, dt = case["op"], case["rows"], case["cols"], TYPES[case["type"]]
+    code = emac.dtype_code(dt)
+    if op == "ckpt8":
+        q, sc = _saved(case)
+        out = {"x": _empty(case)}
+        save = emac.save8_init(rows, cols, code, i["x"].data_ptr(), q.data_ptr(), sc.data_ptr(), x_stride=i["x"].stride(0), q_stride=q.stride(0))
+        back = emac.restore8_init(rows, cols, code, q.data_ptr(), sc.data_ptr(), out["x"].data_ptr(), q_stride=q.stride(0))
+        return out, _Handles(save, back), (q, sc)
+    if op == "act8":
+        kind = {"silu": emac.SILU, "gelu": emac.GELU, "gelu_tanh": emac.GELU_TANH}[case["act"]]
+        qa, sa = _saved(case)
+        out = {"h": _empty(case), "da": _empty(case)}
+        fwd, bwd, qb, sb = {}, {}, None, None
+        if case["gate"]:
+            qb, sb = _saved(case)
+            ab = _empty(case, 2 * cols)
+            out["da"], out["db"] = ab[:, :cols], ab[:, cols:]
+            fwd = {"b": i["b"].data_ptr(), "b_stride": i["b"].stride(0), "qb": qb.data_ptr(), "sb": sb.data_ptr()}
+            bwd = {"db": out["db"].data_ptr(), "db_stride": out["db"].stride(0), "qb": qb.data_ptr(), "sb": sb.data_ptr()}
+        f = emac.act_init(rows, cols, code, kind, i["a"].data_ptr(), out["h"].data_ptr(), a_stride=i["a"].stride(0), qa=qa.data_ptr(), sa=sa.data_ptr(),
+                          q_stride=qa.stride(0), **fwd)
+        b = emac.act_grad_init(rows, cols, code, kind, i["dh"].data_ptr(), qa.data_ptr(), sa.data_ptr(), out["da"].data_ptr(), dh_stride=i["dh"].stride(0),
+                               da_stride=out["da"].stride(0), q_stride=qa.stride(0), **bwd)
+        return out, _Handles(f, b), (qa, sa, qb, sb)
+    out, handles, kept = {}, [], []
+    stats = [torch.empty(rows, device="cuda") for _ in range(2)]
+    kw = {"weight": i["w"].data_ptr(), "wdtype": emac.dtype_code(i["w"].dtype)}
+    q = sc = None
+    if op in ("norm", "step8"):
+        out["y"], out["mean"], out["rstd"] = _empty(case), *stats
+        more = {}
+        if case["residual"]:
+            more.update(residual=i["res"].data_ptr(), residual_stride=i["res"].stride(0))
+        if case["residual"] or case["nsrc"] > 1:
+            out["sum"] = _empty(case)
+            more["sum"] = out["sum"].data_ptr()
+        if op == "step8":
+            q, sc = _saved(case)
+            more.update(q=q.data_ptr(), scale=sc.data_ptr(), q_stride=q.stride(0))
+        handles.append(emac.layernorm_init(rows, cols, code, [t.data_ptr() for t in i["src"]], out["y"].data_ptr(), src_stride=i["src"][0].stride(0),
+                                           bias=i["b"].data_ptr(), eps=EPS, mean=stats[0].data_ptr(), rstd=stats[1].data_ptr(), **kw, **more))
+    if op in ("grad", "step8"):
+        out["dx"] = _empty(case)
+        out["dw"], out["db"] = torch.empty_like(i["w"]), torch.empty_like(i["w"])
+        more = {}
+        if case["residual"]:
+            more.update(dsum=i["dsum"].data_ptr(), dsum_stride=i["dsum"].stride(0))
+        if op == "step8":
+            more.update(q=q.data_ptr(), scale=sc.data_ptr(), q_stride=q.stride(0))
+        else:
+            more.update(x=i["x"].data_ptr(), x_stride=i["x"].stride(0))
+            stats = [i["mean"], i["rstd"]]
+        handles.append(emac.layernorm_grad_init(rows, cols, code, [t.data_ptr() for t in i["dy"]], stats[0].data_ptr(), stats[1].data_ptr(),
+                                                dy_stride=i["dy"][0].stride(0), dx=out["dx"].data_ptr(), dweight=out["dw"].data_ptr(),
+                                                dbias=out["db"].data_ptr(), gdtype=emac.dtype_code(i["w"].dtype), **kw, **more))
+    kept += [q, sc]
+    return out, _Handles(*handles), kept
+
+
+# ---- one pass ----
+
+def run(state):
+    if own:
+        hs = state["handles"]
+        for h in hs.all:
+            hs.start(h)
+        return state["out"]
+    case, i = state["case"], state["in"]
+    return {"norm": _norm, "grad": _grad, "step8": _step8, "ckpt8": _ckpt8, "act8": _act8}[case["op"]](case, i)
+
+
+def _through8(x):
+    """x in 32 bits through 8 bits and back."""
+    rows, cols = x.shape
+    nb = -(-cols // BLOCK)
+    t = torch.zeros(rows, nb * BLOCK, device=x.device)
+    t[:, :cols] = x
+    t = t.view(rows, nb, BLOCK)
+    a = t.abs().amax(2, keepdim=True).clamp_min(TINY)
+    q = torch.round(t * (torch.full_like(a, 127.0) / a)).to(torch.int8)  # a true division: number / tensor is a reciprocal and a product
+    return (q.float() * (a * INV127)).view(rows, nb * BLOCK)[:, :cols]
+
+
+def _ckpt8(case, i):
+    return {"x": _through8(i["x"].float()).to(TYPES[case["type"]])}
+
+
+def _folded(ts):
+    return functools.reduce(torch.add, [t.float() for t in ts])
+
+
+def _norm(case, i):
+    dt = TYPES[case["type"]]
+    s = _folded(i["src"])
+    x = ((s + i["res"].float()) if case["residual"] else s).to(dt)
+    x32 = x.float()
+    mean = x32.sum(1, keepdim=True) / case["cols"]
+    d = x32 - mean
+    rstd = torch.rsqrt(d.square().sum(1, keepdim=True) / case["cols"] + EPS)
+    out = {"y": (d * rstd * i["w"].float() + i["b"].float()).to(dt), "mean": mean[:, 0], "rstd": rstd[:, 0]}
+    if case["residual"] or case["nsrc"] > 1:
+        out["sum"] = x
+    return out
+
+
+def _grad(case, i):
+    return _grad_of(case, i, i["x"].float(), i["mean"], i["rstd"])
+
+
+def _grad_of(case, i, x32, mean, rstd):
+    n = case["cols"]
+    g = _folded(i["dy"])
+    xh = (x32 - mean[:, None]) * rstd[:, None]
+    gw = g * i["w"].float()
+    dx = rstd[:, None] * (gw - gw.sum(1, keepdim=True) / n - xh * ((gw * xh).sum(1, keepdim=True) / n))
+    if case["residual"]:
+        dx = dx + i["dsum"].float()
+    return {"dx": dx.to(TYPES[case["type"]]), "dw": (g * xh).sum(0).to(i["w"].dtype), "db": g.sum(0).to(i["w"].dtype)}
+
+
+def _step8(case, i):
+    out = _norm(case, i)
+    x = out["sum"] if "sum" in out else i["src"][0]
+    return {**out, **_grad_of(case, i, _through8(x.float()), out["mean"], out["rstd"])}
+
+
+def _act_and_slope(act, a):
+    """act(a) and its derivative."""
+    if act == "silu":
+        s = 1 / (1 + torch.exp(-a))
+        return a * s, s * (1 + a * (1 - s))
+    if act == "gelu":
+        p = 0.5 * (1 + torch.erf(a * math.sqrt(0.5)))
+        return a * p, p + a * torch.exp(-0.5 * a * a) * (1 / math.sqrt(2 * math.pi))
+    k = math.sqrt(2 / math.pi)
+    t = torch.tanh(k * (a + 0.044715 * a * a * a))
+    return 0.5 * a * (1 + t), 0.5 * (1 + t) + 0.5 * a * (1 - t * t) * k * (1 + 3 * 0.044715 * a * a)
+
+
+def _act8(case, i):
+    dt = TYPES[case["type"]]
+    a, dh = i["a"].float(), i["dh"].float()
+    v = _act_and_slope(case["act"], a)[0]
+    ra = _through8(a)
+    rv, slope = _act_and_slope(case["act"], ra)
+    if not case["gate"]:
+        return {"h": v.to(dt), "da": (dh * slope).to(dt)}
+    b = i["b"].float()
+    return {"h": (v * b).to(dt), "da": (dh * _through8(b) * slope).to(dt), "db": (dh * rv).to(dt)}
+
+
+# ---- the definitions in 64 bits ----
+
+def _r32(t):
+    """A 64-bit value rounded to 32 bits, where the definition rounds."""
+    return t.float().double()
+
+
+def _restored64(x):
+    """What a checkpoint of x (64 bits, values of the tensors' type) restores to."""
+    rows, cols = x.shape
+    out = torch.empty_like(x)
+    for c in range(0, cols, BLOCK):
+        t = x[:, c:c + BLOCK]
+        a = t.abs().max(dim=1, keepdim=True).values.clamp(min=TINY)
+        q = _r32(t * _r32(torch.full_like(a, 127.0).div(a))).round()
+        out[:, c:c + BLOCK] = _r32(q * _r32(a * INV127))
+    return out
+
+
+def _rounded64(t, case):
+    return t.to(torch.float32).to(TYPES[case["type"]]).double()
+
+
+def _norm64(case, i):
+    t = i["src"][0].double()
+    for s in i["src"][1:]:  # the fold's additions are rounded to 32 bits: the sum is exact bit by bit
+        t = _r32(t + s.double())
+    if case["residual"]:
+        t = _r32(t + i["res"].double())
+    x = _rounded64(t, case)
+    mean = x.mean(dim=1)
+    rstd = (x.var(dim=1, unbiased=False) + EPS).pow(-0.5)
+    xh = (x - mean.unsqueeze(1)) * rstd.unsqueeze(1)
+    out = {"y": torch.addcmul(i["b"].double(), xh, i["w"].double()), "mean": mean, "rstd": rstd}
+    if case["residual"] or case["nsrc"] > 1:
+        out["sum"] = x
+    return x, out
+
+
+def _grad64(case, i, x, mean, rstd):
+    g = sum(t.double() for t in i["dy"])
+    xh = (x - mean.unsqueeze(1)).mul_(rstd.unsqueeze(1))
+    db, dw = g.sum(dim=0), (g * xh).sum(dim=0)
+    g = g * i["w"].double()
+    dx = g - g.mean(dim=1, keepdim=True) - xh * (g * xh).mean(dim=1, keepdim=True)
+    dx *= rstd.unsqueeze(1)
+    if case["residual"]:
+        dx += i["dsum"].double()
+    return {"dx": dx, "dw": dw, "db": db}
+
+
+def _value64(act, a):
+    if act == "silu":
+        return a * torch.sigmoid(a)
+    if act == "gelu":
+        return a * torch.special.ndtr(a)
+    return a * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (a + 0.044715 * a ** 3))
+
+
+def _slope64(act, a):
+    if act == "silu":
+        s = torch.sigmoid(a)
+        return s + a * s * torch.sigmoid(-a)
+    if act == "gelu":
+        return torch.special.ndtr(a) + a * torch.exp(-a ** 2 / 2) / math.sqrt(2 * math.pi)
+    k = 2 * math.sqrt(2 / math.pi)
+    u = k * (a + 0.044715 * a ** 3)
+    return torch.sigmoid(u) + a * torch.sigmoid(u) * torch.sigmoid(-u) * k * (1 + 0.134145 * a ** 2)
+
+
+def exact(case, seed):
+    i, op = _inputs(case, seed), case["op"]
+    if op == "ckpt8":
+        return {"x": _restored64(i["x"].double())}
+    if op == "act8":
+        a, dh = i["a"].double(), i["dh"].double()
+        ra = _restored64(a)
+        h, da = _value64(case["act"], a), dh * _slope64(case["act"], ra)
+        if not case["gate"]:
+            return {"h": h, "da": da}
+        b = i["b"].double()
+        return {"h": h * b, "da": da * _restored64(b), "db": dh * _value64(case["act"], ra)}
+    if op == "grad":
+        return _grad64(case, i, i["x"].double(), i["mean"].double(), i["rstd"].double())
+    x, out = _norm64(case, i)
+    if op == "step8":
+        out = {**out, **_grad64(case, i, _restored64(x), out["mean"], out["rstd"])}
+    return out
