@@ -19,6 +19,7 @@ LIB_PATH = os.environ.get("EXT_MPI_AMD_LIB") or os.path.join(HERE, "libext_mpi_a
 MPI_LIB_PATH = os.path.join(HERE, "libext_mpi_collectives.so")
 
 DOUBLE, LONG, FLOAT, INT = 0, 1, 2, 3
+BF16, HALF = 4, 5  # the row operators (layernorm_init and below) alone
 SUM, MIN, MAX = 0, 1, 2  # element operations (include/ext_mpi_amd.h EXT_MPI_AMD_SUM / _MIN / _MAX)
 UNIQUE_ID_BYTES = 128
 MAX_RANKS = 16
@@ -28,8 +29,9 @@ ERRORS = {-1: "ERROR_MALLOC", -2: "ERROR_SHMEM", -3: "ERROR_ARG", -4: "ERROR_UNS
 ERROR_MALLOC, ERROR_SHMEM, ERROR_ARG, ERROR_UNSUPPORTED, ERROR_DEVICE, ERROR_TRANSPORT = -1, -2, -3, -4, -5, -6
 
 _TORCH_DTYPE_CODES = {"torch.float32": FLOAT, "torch.float64": DOUBLE, "torch.int32": INT,
-                      "torch.int64": LONG}
-_NUMPY_DTYPE_CODES = {"float32": FLOAT, "float64": DOUBLE, "int32": INT, "int64": LONG}
+                      "torch.int64": LONG, "torch.bfloat16": BF16, "torch.float16": HALF}
+_NUMPY_DTYPE_CODES = {"float32": FLOAT, "float64": DOUBLE, "int32": INT, "int64": LONG,
+                      "float16": HALF}
 
 
 class P2P(ctypes.Structure):
@@ -48,6 +50,44 @@ BUF_SEND, BUF_RECV, BUF_STAGE = 0, 1, 2
 # int (*)(void *ctx, const void *send, void *recv, long bytes) -- include/ext_mpi_amd.h
 ALLGATHER_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_long)
 _ipc_callbacks = {}  # comm -> the ctypes callback (must outlive the communicator)
+
+
+SILU, GELU, GELU_TANH = 0, 1, 2  # include/ext_mpi_amd.h EXT_MPI_AMD_SILU / _GELU / _GELU_TANH
+BLOCK8 = 128            # columns that share a checkpoint's scale
+ROW_COLS_MAX = 65536    # layer norm: columns
+_P, _L, _I = ctypes.c_void_p, ctypes.c_long, ctypes.c_int
+_LEAVES = ctypes.c_void_p * MAX_RANKS
+
+
+class LayernormDesc(ctypes.Structure):
+    """include/ext_mpi_amd.h ext_mpi_amd_layernorm"""
+    _fields_ = [("rows", _L), ("cols", _L), ("dtype", _I), ("wdtype", _I), ("nsrc", _I), ("pad_", _I), ("src", _LEAVES),
+                ("src_stride", _L), ("residual", _P), ("residual_stride", _L), ("weight", _P), ("bias", _P),
+                ("eps", ctypes.c_double), ("y", _P), ("y_stride", _L), ("sum", _P), ("sum_stride", _L), ("mean", _P),
+                ("rstd", _P), ("q", _P), ("q_stride", _L), ("scale", _P)]
+
+
+class LayernormGradDesc(ctypes.Structure):
+    """include/ext_mpi_amd.h ext_mpi_amd_layernorm_grad"""
+    _fields_ = [("rows", _L), ("cols", _L), ("dtype", _I), ("wdtype", _I), ("gdtype", _I), ("accumulate", _I),
+                ("nsrc", _I), ("pad_", _I), ("dy", _LEAVES), ("dy_stride", _L), ("x", _P), ("x_stride", _L), ("q", _P),
+                ("q_stride", _L), ("scale", _P), ("mean", _P), ("rstd", _P), ("weight", _P), ("bias", _P), ("dsum", _P),
+                ("dsum_stride", _L), ("dx", _P), ("dx_stride", _L), ("dweight", _P), ("dbias", _P), ("y", _P),
+                ("y_stride", _L)]
+
+
+class ActDesc(ctypes.Structure):
+    """include/ext_mpi_amd.h ext_mpi_amd_act"""
+    _fields_ = [("rows", _L), ("cols", _L), ("dtype", _I), ("kind", _I), ("a", _P), ("a_stride", _L), ("b", _P),
+                ("b_stride", _L), ("h", _P), ("h_stride", _L), ("qa", _P), ("qb", _P), ("q_stride", _L), ("sa", _P),
+                ("sb", _P)]
+
+
+class ActGradDesc(ctypes.Structure):
+    """include/ext_mpi_amd.h ext_mpi_amd_act_grad"""
+    _fields_ = [("rows", _L), ("cols", _L), ("dtype", _I), ("kind", _I), ("dh", _P), ("dh_stride", _L), ("qa", _P),
+                ("qb", _P), ("q_stride", _L), ("sa", _P), ("sb", _P), ("da", _P), ("da_stride", _L), ("db", _P),
+                ("db_stride", _L), ("h", _P), ("h_stride", _L)]
 
 
 class ExtMpiError(RuntimeError):
@@ -124,6 +164,13 @@ def lib():
         L.ext_mpi_amd_build_info.restype = ctypes.c_char_p
         L.ext_mpi_amd_handle_join_parts.argtypes = [c_int]
         L.ext_mpi_amd_handle_ipc_flags.argtypes = [c_int]
+        for name, desc in (("layernorm", LayernormDesc), ("layernorm_grad", LayernormGradDesc), ("act", ActDesc),
+                           ("act_grad", ActGradDesc)):
+            getattr(L, f"ext_mpi_amd_{name}_init").argtypes = [P(desc), P(c_int)]
+        L.ext_mpi_amd_save8_init.argtypes = [c_long, c_long, c_int, c_void_p, c_long, c_void_p, c_long, c_void_p,
+                                             P(c_int)]
+        L.ext_mpi_amd_restore8_init.argtypes = [c_long, c_long, c_int, c_void_p, c_long, c_void_p, c_void_p, c_long,
+                                                P(c_int)]
         L.ext_mpi_amd_gpu_malloc.argtypes = [P(c_void_p), ctypes.c_size_t]
         L.ext_mpi_amd_gpu_free.argtypes = [c_void_p]
         L.ext_mpi_amd_gpu_memcpy_hd.argtypes = [c_void_p, c_void_p, ctypes.c_size_t]
@@ -139,7 +186,7 @@ def dtype_code(dt):
         return _TORCH_DTYPE_CODES[key]
     if key in _NUMPY_DTYPE_CODES:
         return _NUMPY_DTYPE_CODES[key]
-    raise ValueError(f"unsupported element type {dt} (float, double, int, long only)")
+    raise ValueError(f"unsupported element type {dt} (float, double, int, long; bfloat16 and half for the row operators)")
 
 
 def _check(what, rc):
@@ -186,6 +233,75 @@ def fold_init(srcptrs, dstptrs, count, dtype, op=SUM):
     _check("ext_mpi_amd_fold_init",
            lib().ext_mpi_amd_fold_init(len(srcptrs), s, len(dstptrs), d, count, dtype, op, ctypes.byref(h)))
     return h.value
+
+
+def _leaves(ptrs):
+    if not 1 <= len(ptrs) <= MAX_RANKS:
+        raise ValueError(f"{len(ptrs)} leaves (1 to {MAX_RANKS})")
+    return _LEAVES(*ptrs)
+
+
+def _row_init(name, desc):
+    h = ctypes.c_int(-1)
+    _check(f"ext_mpi_amd_{name}_init", getattr(lib(), f"ext_mpi_amd_{name}_init")(ctypes.byref(desc), ctypes.byref(h)))
+    return h.value
+
+
+def layernorm_init(rows, cols, dtype, srcptrs, y=None, *, src_stride=0, y_stride=0, residual=None, residual_stride=0,
+                   weight=None, bias=None, wdtype=None, eps=1e-5, sum=None, sum_stride=0, mean=None, rstd=None, q=None,
+                   q_stride=0, scale=None):
+    """Persistent layer norm of the rows of x = ((src0 + src1) + ...) + residual (device addresses;
+    strides in elements, 0: contiguous): y, and what is asked for of x itself (sum), the statistics
+    the gradient takes (mean, rstd: floats) and a checkpoint of x in 8 bits (q, scale). wdtype:
+    the type of weight and bias, dtype (the default) or FLOAT."""
+    return _row_init("layernorm", LayernormDesc(
+        rows, cols, dtype, dtype if wdtype is None else wdtype, len(srcptrs), 0, _leaves(srcptrs), src_stride, residual,
+        residual_stride, weight, bias, eps, y, y_stride, sum, sum_stride, mean, rstd, q, q_stride, scale))
+
+
+def layernorm_grad_init(rows, cols, dtype, dyptrs, mean, rstd, *, dy_stride=0, x=None, x_stride=0, q=None, q_stride=0,
+                        scale=None, weight=None, bias=None, wdtype=None, dsum=None, dsum_stride=0, dx=None, dx_stride=0,
+                        dweight=None, dbias=None, gdtype=None, accumulate=False, y=None, y_stride=0):
+    """Persistent gradient of layernorm_init for the folded gradients dy0 + dy1 + ..., from x or from
+    its checkpoint (q, scale): dx (plus dsum), dweight and dbias (added to with ``accumulate``), and
+    the norm's output y again if asked for."""
+    return _row_init("layernorm_grad", LayernormGradDesc(
+        rows, cols, dtype, dtype if wdtype is None else wdtype, dtype if gdtype is None else gdtype, bool(accumulate),
+        len(dyptrs), 0, _leaves(dyptrs), dy_stride, x, x_stride, q, q_stride, scale, mean, rstd, weight, bias, dsum,
+        dsum_stride, dx, dx_stride, dweight, dbias, y, y_stride))
+
+
+def save8_init(rows, cols, dtype, x, q, scale, *, x_stride=0, q_stride=0):
+    """Persistent checkpoint of x in 8 bits: q (rows x cols bytes) and scale (rows x ceil(cols / 128)
+    floats); x restores as q * scale."""
+    h = ctypes.c_int(-1)
+    _check("ext_mpi_amd_save8_init", lib().ext_mpi_amd_save8_init(rows, cols, dtype, x, x_stride, q, q_stride, scale,
+                                                                  ctypes.byref(h)))
+    return h.value
+
+
+def restore8_init(rows, cols, dtype, q, scale, x, *, q_stride=0, x_stride=0):
+    """Persistent restoration of a checkpoint into x."""
+    h = ctypes.c_int(-1)
+    _check("ext_mpi_amd_restore8_init", lib().ext_mpi_amd_restore8_init(rows, cols, dtype, q, q_stride, scale, x,
+                                                                        x_stride, ctypes.byref(h)))
+    return h.value
+
+
+def act_init(rows, cols, dtype, kind, a, h=None, *, b=None, a_stride=0, b_stride=0, h_stride=0, qa=None, sa=None, qb=None,
+             sb=None, q_stride=0):
+    """Persistent activation h = f(a), or f(a) * b with a gate (kind: SILU, GELU, GELU_TANH), with
+    checkpoints of a (qa, sa) and b (qb, sb) if asked for."""
+    return _row_init("act", ActDesc(rows, cols, dtype, kind, a, a_stride, b, b_stride, h, h_stride, qa, qb, q_stride, sa,
+                                    sb))
+
+
+def act_grad_init(rows, cols, dtype, kind, dh, qa, sa, da, *, qb=None, sb=None, db=None, dh_stride=0, da_stride=0,
+                  db_stride=0, q_stride=0, h=None, h_stride=0):
+    """Persistent gradient of act_init from its checkpoints: da, with a gate db, and h again if
+    asked for."""
+    return _row_init("act_grad", ActGradDesc(rows, cols, dtype, kind, dh, dh_stride, qa, qb, q_stride, sa, sb, da,
+                                             da_stride, db, db_stride, h, h_stride))
 
 
 def get_unique_id():

@@ -1,0 +1,334 @@
+// act8.hip -- activations with 8-bit checkpoints of their inputs, their gradient from the
+// checkpoints, and the checkpoints alone.
+//
+// Everything here is one pass over HBM: a 16-lane group owns one checkpoint block (128 columns of
+// one row), kUnroll groups' loads are issued before the first is used, and a block's maximum is a
+// reduction inside the group, so nothing is read twice and no barrier is needed. Blocks are
+// numbered row by row; a workgroup divides once (scalars) and a lane only where a row holds fewer
+// blocks than a workgroup takes. Bound by HBM; the arithmetic is about 30 lane operations per
+// element, of the 50 or so that fit beside 8 bytes of traffic.
+#include "rows_kernel.hpp"
+
+namespace {
+
+using namespace emac_rows;
+
+constexpr int kUnroll = 4, kGroups = 16; // blocks a lane group takes, groups in a workgroup
+
+// ---- activations: value and slope, in 32 bits ----
+// 16-bit types take the native exp2 and reciprocal (1 ulp each); float the library's exp and IEEE
+// division, since 2 ulp of the native ones' argument rounding would show in its far tails.
+template <class T>
+__device__ inline float exp_of(float x) {
+  return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f);
+}
+template <>
+__device__ inline float exp_of<float>(float x) {
+  return expf(x);
+}
+template <class T>
+__device__ inline float recip(float x) {
+  return __builtin_amdgcn_rcpf(x);
+}
+template <>
+__device__ inline float recip<float>(float x) {
+  return 1.0f / x;
+}
+
+template <class T, int KIND>
+__device__ inline float act_value(float a) {
+  if constexpr (KIND == EXT_MPI_AMD_SILU) {
+    return a * recip<T>(1.0f + exp_of<T>(-a));
+  } else if constexpr (KIND == EXT_MPI_AMD_GELU_TANH) {
+    // (1 + tanh u) / 2 = 1 / (1 + exp(-2u)); beyond |a| = 64 it is 0 or 1 in 32 bits
+    const float c = __builtin_amdgcn_fmed3f(a, -64.0f, 64.0f);
+    const float u = 1.5957691216057308f * c * (1.0f + 0.044715f * c * c);
+    return a * recip<T>(1.0f + exp_of<T>(-u));
+  } else {
+    float e, p;
+    // the normal distribution's tail, p = exp(-a^2/2) erfcx(|a|/sqrt 2) / 2, with erfcx(z) as a
+    // polynomial of degree 8 in t = 1 / (1 + 0.4348731 z) without a constant term (least relative
+    // error on 0 <= z <= 12, fitted here: 1.3e-7)
+    const float t = recip<T>(1.0f + 0.30750170f * fabsf(a));
+    e = exp_of<T>(-0.5f * a * a);
+    p = 0.036300003528594971f;
+    p = p * t - 0.14733710885047913f;
+    p = p * t + 0.1701858937740326f;
+    p = p * t - 0.026046559214591980f;
+    p = p * t + 0.1153081208467484f;
+    p = p * t + 0.1056915521621704f;
+    p = p * t + 0.1232480555772781f;
+    p = p * t + 0.1226501166820526f;
+    p = p * t * e;
+    return a * (a > 0.0f ? 1.0f - p : p);
+  }
+}
+
+template <class T, int KIND>
+__device__ inline void act_both(float a, float &value, float &slope) {
+  if constexpr (KIND == EXT_MPI_AMD_SILU) {
+    const float s = recip<T>(1.0f + exp_of<T>(-a));
+    value = a * s;
+    slope = s * (1.0f + a * (1.0f - s));
+  } else if constexpr (KIND == EXT_MPI_AMD_GELU_TANH) {
+    const float c = __builtin_amdgcn_fmed3f(a, -64.0f, 64.0f), c2 = 0.044715f * c * c;
+    const float s = recip<T>(1.0f + exp_of<T>(-1.5957691216057308f * c * (1.0f + c2)));
+    value = a * s;
+    slope = s + value * (1.0f - s) * (1.5957691216057308f * (1.0f + 3.0f * c2));
+  } else {
+    const float t = recip<T>(1.0f + 0.30750170f * fabsf(a));
+    const float e = exp_of<T>(-0.5f * a * a);
+    float p = 0.036300003528594971f;
+    p = p * t - 0.14733710885047913f;
+    p = p * t + 0.1701858937740326f;
+    p = p * t - 0.026046559214591980f;
+    p = p * t + 0.1153081208467484f;
+    p = p * t + 0.1056915521621704f;
+    p = p * t + 0.1232480555772781f;
+    p = p * t + 0.1226501166820526f;
+    p = p * t * e;
+    const float phi = a > 0.0f ? 1.0f - p : p;
+    value = a * phi;
+    slope = phi + a * e * 0.3989422804014327f;
+  }
+}
+
+// where a lane's 8 elements of block `u` (0 .. kUnroll - 1) of its group lie
+struct place {
+  long row;
+  int blk, c; // block of the row, first column of the lane
+  long n;     // elements from there to the row's end, 0 or less if none
+};
+struct span8 {
+  long row0;
+  unsigned blk0, nblk;
+  long rows, cols;
+  __device__ span8(long rows_, long cols_, unsigned nblk_) : nblk(nblk_), rows(rows_), cols(cols_) {
+    const unsigned first = blockIdx.x * (unsigned)(kUnroll * kGroups);
+    row0 = first / nblk;
+    blk0 = first - (unsigned)row0 * nblk;
+  }
+  __device__ place at(int u) const {
+    const unsigned x = blk0 + u * kGroups + threadIdx.x / 16;
+    place p;
+    unsigned k;
+    if (nblk >= (unsigned)(kUnroll * kGroups)) k = x >= nblk ? 1u : 0u;
+    else k = x / nblk;
+    p.row = row0 + k;
+    p.blk = (int)(x - k * nblk);
+    p.c = p.blk * EMAC_BLOCK8 + (int)(threadIdx.x % 16) * 8;
+    p.n = p.row < rows ? cols - p.c : 0;
+    return p;
+  }
+};
+
+template <class T>
+__device__ inline void put8(const place &p, v8<T> x, signed char *q, long q_stride, float *scale, unsigned nblk) {
+  const block8 b = quantise<T>(x);
+  if (p.n > 0) {
+    store8q(q + p.row * q_stride + p.c, b.q, p.n);
+    if (threadIdx.x % 16 == 0) scale[p.row * nblk + p.blk] = b.scale;
+  }
+}
+
+template <class T, int KIND, bool GATE>
+__global__ __launch_bounds__(256) void act_kernel(const ext_mpi_amd_act d, unsigned nblk) {
+  const span8 s(d.rows, d.cols, nblk);
+  v8<T> a[kUnroll], b[GATE ? kUnroll : 1];
+#pragma unroll
+  for (int u = 0; u < kUnroll; u++) {
+    const place p = s.at(u);
+    a[u] = (v8<T>)(T)0;
+    if (GATE) b[GATE ? u : 0] = a[u];
+    if (p.n > 0) {
+      a[u] = load8((const T *)d.a + p.row * d.a_stride + p.c, p.n);
+      if (GATE) b[GATE ? u : 0] = load8((const T *)d.b + p.row * d.b_stride + p.c, p.n);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; u++) {
+    const place p = s.at(u);
+    if (d.qa) {
+      put8<T>(p, a[u], d.qa, d.q_stride, d.sa, nblk);
+      if (GATE) put8<T>(p, b[GATE ? u : 0], d.qb, d.q_stride, d.sb, nblk);
+    }
+    if constexpr (KIND != EMAC_SAVE8) {
+      if (d.h && p.n > 0) {
+        const f8 f = widen<T>(a[u]);
+        f8 v;
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = act_value<T, KIND>(f[j]);
+        if (GATE) v *= widen<T>(b[GATE ? u : 0]);
+        store8((T *)d.h + p.row * d.h_stride + p.c, round_to<T>(v), p.n);
+      }
+    }
+  }
+}
+
+template <class T, int KIND, bool GATE>
+__global__ __launch_bounds__(256) void act_grad_kernel(const ext_mpi_amd_act_grad d, unsigned nblk) {
+  const span8 s(d.rows, d.cols, nblk);
+  v8<T> g[kUnroll];
+  u2 qa[kUnroll], qb[GATE ? kUnroll : 1];
+  float sa[kUnroll], sb[GATE ? kUnroll : 1];
+#pragma unroll
+  for (int u = 0; u < kUnroll; u++) {
+    const place p = s.at(u);
+    if (p.n > 0) {
+      g[u] = load8((const T *)d.dh + p.row * d.dh_stride + p.c, p.n);
+      qa[u] = load8q(d.qa + p.row * d.q_stride + p.c, p.n);
+      sa[u] = d.sa[p.row * nblk + p.blk];
+      if (GATE) {
+        qb[GATE ? u : 0] = load8q(d.qb + p.row * d.q_stride + p.c, p.n);
+        sb[GATE ? u : 0] = d.sb[p.row * nblk + p.blk];
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; u++) {
+    const place p = s.at(u);
+    if (p.n <= 0) continue;
+    const f8 a = restore(qa[u], sa[u]), dh = widen<T>(g[u]);
+    f8 value, slope;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      float v, w;
+      act_both<T, KIND>(a[j], v, w);
+      value[j] = v;
+      slope[j] = w;
+    }
+    slope *= dh;
+    if (GATE) {
+      const f8 b = restore(qb[GATE ? u : 0], sb[GATE ? u : 0]);
+      store8((T *)d.da + p.row * d.da_stride + p.c, round_to<T>(slope * b), p.n);
+      store8((T *)d.db + p.row * d.db_stride + p.c, round_to<T>(dh * value), p.n);
+      value *= b;
+    } else {
+      store8((T *)d.da + p.row * d.da_stride + p.c, round_to<T>(slope), p.n);
+    }
+    if (d.h) store8((T *)d.h + p.row * d.h_stride + p.c, round_to<T>(value), p.n);
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void restore8_kernel(long rows, long cols, const signed char *q, long q_stride,
+                                                       const float *scale, T *x, long x_stride, unsigned nblk) {
+  const span8 s(rows, cols, nblk);
+  u2 w[kUnroll];
+  float sc[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; u++) {
+    const place p = s.at(u);
+    if (p.n > 0) {
+      w[u] = load8q(q + p.row * q_stride + p.c, p.n);
+      sc[u] = scale[p.row * nblk + p.blk];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; u++) {
+    const place p = s.at(u);
+    if (p.n > 0) store8(x + p.row * x_stride + p.c, round_to<T>(restore(w[u], sc[u])), p.n);
+  }
+}
+
+// ---- launches ----
+
+struct grid8 {
+  unsigned nblk, grid;
+};
+// blocks and workgroups of a matrix (engine_rows.c holds rows * blocks under 2^31)
+grid8 grid_of(long rows, long cols) {
+  grid8 g;
+  g.nblk = (unsigned)((cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8);
+  g.grid = (unsigned)((rows * g.nblk + kUnroll * kGroups - 1) / (kUnroll * kGroups));
+  return g;
+}
+
+template <class T, int KIND>
+int act_go(const ext_mpi_amd_act &d, hipStream_t st) {
+  const grid8 g = grid_of(d.rows, d.cols);
+  if (d.b) act_kernel<T, KIND, true><<<g.grid, 256, 0, st>>>(d, g.nblk);
+  else act_kernel<T, KIND, false><<<g.grid, 256, 0, st>>>(d, g.nblk);
+  return launched();
+}
+
+template <class T>
+int act_t(const ext_mpi_amd_act &d, hipStream_t st) {
+  switch (d.kind) {
+  case EMAC_SAVE8: {
+    const grid8 g = grid_of(d.rows, d.cols);
+    act_kernel<T, EMAC_SAVE8, false><<<g.grid, 256, 0, st>>>(d, g.nblk);
+    return launched();
+  }
+  case EXT_MPI_AMD_SILU: return act_go<T, EXT_MPI_AMD_SILU>(d, st);
+  case EXT_MPI_AMD_GELU: return act_go<T, EXT_MPI_AMD_GELU>(d, st);
+  case EXT_MPI_AMD_GELU_TANH: return act_go<T, EXT_MPI_AMD_GELU_TANH>(d, st);
+  }
+  return EMAC_ERR_ARG;
+}
+
+template <class T, int KIND>
+int act_grad_go(const ext_mpi_amd_act_grad &d, hipStream_t st) {
+  const grid8 g = grid_of(d.rows, d.cols);
+  if (d.qb) act_grad_kernel<T, KIND, true><<<g.grid, 256, 0, st>>>(d, g.nblk);
+  else act_grad_kernel<T, KIND, false><<<g.grid, 256, 0, st>>>(d, g.nblk);
+  return launched();
+}
+
+template <class T>
+int act_grad_t(const ext_mpi_amd_act_grad &d, hipStream_t st) {
+  switch (d.kind) {
+  case EXT_MPI_AMD_SILU: return act_grad_go<T, EXT_MPI_AMD_SILU>(d, st);
+  case EXT_MPI_AMD_GELU: return act_grad_go<T, EXT_MPI_AMD_GELU>(d, st);
+  case EXT_MPI_AMD_GELU_TANH: return act_grad_go<T, EXT_MPI_AMD_GELU_TANH>(d, st);
+  }
+  return EMAC_ERR_ARG;
+}
+
+template <class T>
+int restore_t(long rows, long cols, const signed char *q, long q_stride, const float *scale, void *x, long x_stride,
+              hipStream_t st) {
+  const grid8 g = grid_of(rows, cols);
+  restore8_kernel<T><<<g.grid, 256, 0, st>>>(rows, cols, q, q_stride, scale, (T *)x, x_stride, g.nblk);
+  return launched();
+}
+
+} // namespace
+
+extern "C" {
+
+int emac_gpu_act(const ext_mpi_amd_act *d, void *stream) {
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (d->rows <= 0) return 0;
+  switch (d->dtype) {
+  case EXT_MPI_AMD_FLOAT: return act_t<float>(*d, st);
+  case EXT_MPI_AMD_BF16: return act_t<bf16>(*d, st);
+  case EXT_MPI_AMD_HALF: return act_t<half>(*d, st);
+  }
+  return EMAC_ERR_UNSUPPORTED;
+}
+
+int emac_gpu_act_grad(const ext_mpi_amd_act_grad *d, void *stream) {
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (d->rows <= 0) return 0;
+  switch (d->dtype) {
+  case EXT_MPI_AMD_FLOAT: return act_grad_t<float>(*d, st);
+  case EXT_MPI_AMD_BF16: return act_grad_t<bf16>(*d, st);
+  case EXT_MPI_AMD_HALF: return act_grad_t<half>(*d, st);
+  }
+  return EMAC_ERR_UNSUPPORTED;
+}
+
+int emac_gpu_restore8(long rows, long cols, int dtype, const signed char *q, long q_stride, const float *scale, void *x,
+                      long x_stride, void *stream) {
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (rows <= 0) return 0;
+  switch (dtype) {
+  case EXT_MPI_AMD_FLOAT: return restore_t<float>(rows, cols, q, q_stride, scale, x, x_stride, st);
+  case EXT_MPI_AMD_BF16: return restore_t<bf16>(rows, cols, q, q_stride, scale, x, x_stride, st);
+  case EXT_MPI_AMD_HALF: return restore_t<half>(rows, cols, q, q_stride, scale, x, x_stride, st);
+  }
+  return EMAC_ERR_UNSUPPORTED;
+}
+
+} // extern "C"

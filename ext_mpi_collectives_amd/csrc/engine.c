@@ -45,8 +45,9 @@ static int new_handle_slot(void) {
 void handle_release(emac_handle *h) {
   int r;
   if (!h) return;
+  rows_free(h); /* a row operator: its Start waited for, its workspace */
   if (h->stream) {
-    emac_gpu_stream_sync(h->stream);
+    if (h->kind != KIND_ROWS) emac_gpu_stream_sync(h->stream);
     if (h->own_stream) emac_gpu_stream_destroy(h->stream);
   }
   emac_gpu_free(h->d_buckets);
@@ -402,6 +403,10 @@ int ext_mpi_amd_start_legs(int handle, int legs) {
   emac_handle *h = handle_get(handle);
   int rc, key;
   if (!h) return EMAC_ERR_ARG;
+  if (h->rows) { /* one leg: the computation */
+    if (legs >> EMAC_LEG_STEP_SHIFT) return EMAC_ERR_ARG;
+    return (legs & EXT_MPI_AMD_LEG_FOLD) ? rows_start(h) : 0;
+  }
   if (emac_gpu_set_device(h->device)) return EMAC_ERR_DEVICE;
   key = legs & EXT_MPI_AMD_LEG_ALL;
   if (legs >> EMAC_LEG_STEP_SHIFT) { /* one node step alone (loopback lock-step): never captured */
@@ -434,6 +439,7 @@ int ext_mpi_amd_start(int handle) { return ext_mpi_amd_start_legs(handle, EXT_MP
 
 int ext_mpi_amd_set_stream(int handle, void *stream) {
   emac_handle *h = handle_get(handle);
+  if (h && h->rows) return rows_set_stream(h, stream);
   if (!h || !stream) return EMAC_ERR_ARG;
   emac_gpu_stream_sync(h->stream);
   if (h->own_stream) emac_gpu_stream_destroy(h->stream);
@@ -459,6 +465,7 @@ int ext_mpi_amd_wait(int handle) {
   emac_handle *h = handle_get(handle);
   int rc;
   if (!h) return EMAC_ERR_ARG;
+  if (h->rows && !h->started) return 0;
   rc = emac_gpu_stream_sync(h->stream);
   h->started = 0;
   return rc ? rc : ipc_status(h);
@@ -484,6 +491,7 @@ int ext_mpi_amd_done(int handle) {
 
 void *ext_mpi_amd_stream(int handle) {
   emac_handle *h = handle_get(handle);
+  if (h && h->rows && rows_stream(h)) return NULL;
   return h ? h->stream : NULL;
 }
 

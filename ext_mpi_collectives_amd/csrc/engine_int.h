@@ -6,6 +6,7 @@
  *   engine.c       handle table, buffer mapping, bucket upload, Start / Test / Wait / Done
  *   engine_tune.c  per-handle launch-schedule tuning of the fold, and the per-process cache of
  *                  tuned schedules shared by handles of one shape
+ *   engine_rows.c  the row operators (layer norm, 8-bit checkpoints)
  *   engine_node.c  NODE form (every node rank in this process), the layout self-check
  *   engine_comm.c  COMM form over RCCL (and the loopback test transport), the point-to-point legs
  *   engine_ipc.c   peer-mapped form (hipIpc over xGMI): mappings, the arena, node barriers
@@ -31,7 +32,7 @@
 #define MAX_HANDLES 4096
 #define MAX_COMMS 64
 
-enum { KIND_NODE = 1, KIND_COMM = 2, KIND_IPC = 3 };
+enum { KIND_NODE = 1, KIND_COMM = 2, KIND_IPC = 3, KIND_ROWS = 4 };
 
 /* one peer allocation mapped into this process (hipIpcOpenMemHandle), shared by every handle and
    communicator that references the same allocation (the exporter's handle bytes, allocation id
@@ -286,6 +287,7 @@ typedef struct {
   size_t part_bytes;
   emac_codes xcodes; /* ... and its share fold's tree (a left fold, or pairs for the halving flow) */
   emac_join *join;   /* ... pipelined by parts, or NULL (the serial join) */
+  struct emac_rows *rows; /* KIND_ROWS: a row operator (engine_rows.c), and nothing of the above but stream */
 } emac_handle;
 
 #define EMAC_IPC_ATTEMPTS 8 /* set-up rounds of a peer-mapped exchange before it gives up */
@@ -308,6 +310,12 @@ int upload_launch(const emac_handle *h, emac_launch *L, emac_bucket *b, int nb);
 int upload_launch_fan(const emac_handle *h, emac_launch *L, emac_bucket *b, int nb, int nsrc, int fan);
 int stage_in(emac_handle *h);
 int stage_out(emac_handle *h);
+
+/* engine_rows.c */
+int rows_stream(emac_handle *h);
+int rows_set_stream(emac_handle *h, void *stream);
+int rows_start(emac_handle *h);
+void rows_free(emac_handle *h);
 
 /* engine_tune.c */
 int upload_buckets(emac_handle *h, emac_bucket *b, int nb);

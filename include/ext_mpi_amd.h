@@ -107,6 +107,133 @@ int ext_mpi_amd_allreduce_init(const void *sendbuf, void *recvbuf, long count, i
 int ext_mpi_amd_comm_malloc(int comm, void **p, unsigned long bytes);
 int ext_mpi_amd_comm_mfree(int comm, void *p);
 
+/* ---- row operators: layer norm over the folded partials of the ranks, its gradient, activation
+ * checkpoints in 8 bits (no reference counterpart) ----
+ * Matrices are rows x cols, row r starting at element r * stride (stride 0: cols, contiguous; else
+ * >= cols), device memory of one device, aligned to their element only; a pointer that is not
+ * "optional" is required unless rows is 0. Element types FLOAT, BF16 and HALF (the Allreduce
+ * handles take neither of the latter two). Everything is computed in 32 bits and rounded once to
+ * the type it is stored in. Handles run, wait and are released as every other handle
+ * (ext_mpi_amd_start / _test / _wait / _done); one Start of a handle is in flight at a time (a
+ * gradient handle owns a workspace), also across graphs that captured its Start; such a graph must
+ * not be replayed after Done, and the stream to capture on is set (ext_mpi_amd_set_stream) before
+ * the capture begins. set_stream also takes the default stream (NULL) here, and Start leaves the
+ * caller's current device as it was. No Start allocates or waits.
+ * An output may be one of the inputs of the same type, in place (same address and stride), except
+ * layernorm_grad's y; any other overlap with an output is EXT_MPI_AMD_ERROR_ARG, as are negative
+ * sizes, short strides, misaligned, host or foreign-device pointers. */
+#define EXT_MPI_AMD_BF16 4
+#define EXT_MPI_AMD_HALF 5
+#define EXT_MPI_AMD_ROW_COLS_MAX 65536 /* layer norm: columns (above: EXT_MPI_AMD_ERROR_UNSUPPORTED) */
+#define EXT_MPI_AMD_BLOCK8 128         /* columns that share a checkpoint's scale */
+
+/* A checkpoint of a rows x cols matrix: q, rows x cols signed bytes (row stride q_stride >= cols, 0:
+ * cols), and scale, rows x ceil(cols / 128) floats, contiguous. For each block of 128 columns,
+ * a = max(max |x|, 2^-100), q = rint(x * (127 / a)) (ties to even), scale = a * (1 / 127); x restores
+ * as q * scale, off by at most a / 254 and a few roundings. A block that holds an infinity or a NaN
+ * restores as NaN throughout. */
+
+/* Layer norm over the rows of x = ((src[0] + src[1]) + ...) + residual, added in 32 bits in that
+ * order and rounded to dtype: y = (x - mean) / sqrt(var + eps) * weight + bias. */
+typedef struct {
+  long rows, cols;
+  int dtype;         /* src, residual, sum, y */
+  int wdtype;        /* weight, bias: dtype or FLOAT */
+  int nsrc;          /* 1 .. EXT_MPI_AMD_MAX_RANKS leaves */
+  int pad_;
+  const void *src[EXT_MPI_AMD_MAX_RANKS];
+  long src_stride;   /* of every leaf */
+  const void *residual; /* optional */
+  long residual_stride;
+  const void *weight, *bias; /* cols elements; optional (1 and 0) */
+  double eps;
+  void *y;           /* optional if sum or q is given */
+  long y_stride;
+  void *sum;         /* optional: x */
+  long sum_stride;
+  float *mean, *rstd; /* rows floats; optional: what the gradient takes */
+  signed char *q;    /* optional, with scale: a checkpoint of x */
+  long q_stride;
+  float *scale;
+} ext_mpi_amd_layernorm;
+int ext_mpi_amd_layernorm_init(const ext_mpi_amd_layernorm *d, int *handle);
+
+/* Its gradient. g = (dy[0] + dy[1]) + ... in 32 bits, xh = (x - mean) * rstd with x given or restored
+ * from its checkpoint (exactly one of the two):
+ *   dx = rstd * (g w - mean_cols(g w) - xh mean_cols(g w xh)) + dsum
+ *   dweight (+)= sum over the rows of g xh, dbias (+)= sum over the rows of g
+ * The row sums are taken in an order that depends on the shape alone: the same bits every time. */
+typedef struct {
+  long rows, cols;
+  int dtype;         /* dy, x, dsum, dx, y */
+  int wdtype;        /* weight, bias: dtype or FLOAT */
+  int gdtype;        /* dweight, dbias: dtype or FLOAT */
+  int accumulate;    /* 1: dweight and dbias are added to */
+  int nsrc;
+  int pad_;
+  const void *dy[EXT_MPI_AMD_MAX_RANKS];
+  long dy_stride;
+  const void *x;     /* x, or q and scale */
+  long x_stride;
+  const signed char *q;
+  long q_stride;
+  const float *scale;
+  const float *mean, *rstd;
+  const void *weight; /* optional */
+  const void *bias;  /* optional: for y */
+  const void *dsum;  /* optional: the gradient that reaches x past the norm */
+  long dsum_stride;
+  void *dx;          /* optional if dweight or dbias is given */
+  long dx_stride;
+  void *dweight, *dbias; /* optional */
+  void *y;           /* optional: the norm's output again, from x or its checkpoint */
+  long y_stride;
+} ext_mpi_amd_layernorm_grad;
+int ext_mpi_amd_layernorm_grad_init(const ext_mpi_amd_layernorm_grad *d, int *handle);
+
+/* x into a checkpoint, and a checkpoint into x (rounded to dtype). */
+int ext_mpi_amd_save8_init(long rows, long cols, int dtype, const void *x, long x_stride, signed char *q, long q_stride,
+                           float *scale, int *handle);
+int ext_mpi_amd_restore8_init(long rows, long cols, int dtype, const signed char *q, long q_stride, const float *scale,
+                              void *x, long x_stride, int *handle);
+
+/* h = f(a), or f(a) * b with a gate b, and checkpoints of a and b for the gradient. */
+#define EXT_MPI_AMD_SILU 0      /* a / (1 + exp(-a)) */
+#define EXT_MPI_AMD_GELU 1      /* a (1 + erf(a / sqrt 2)) / 2 */
+#define EXT_MPI_AMD_GELU_TANH 2 /* a (1 + tanh(sqrt(2 / pi) (a + 0.044715 a^3))) / 2 */
+typedef struct {
+  long rows, cols;
+  int dtype, kind;
+  const void *a;
+  long a_stride;
+  const void *b;     /* optional */
+  long b_stride;
+  void *h;           /* optional if qa is given */
+  long h_stride;
+  signed char *qa, *qb; /* optional: checkpoints of a and (with b) of b, one stride for both */
+  long q_stride;
+  float *sa, *sb;
+} ext_mpi_amd_act;
+int ext_mpi_amd_act_init(const ext_mpi_amd_act *d, int *handle);
+
+/* The gradient from the checkpoints: da = dh f'(a) (times b), db = dh f(a); h again if asked for. */
+typedef struct {
+  long rows, cols;
+  int dtype, kind;
+  const void *dh;
+  long dh_stride;
+  const signed char *qa, *qb; /* qb, sb and db: with a gate */
+  long q_stride;
+  const float *sa, *sb;
+  void *da;          /* required */
+  long da_stride;
+  void *db;          /* required with a gate */
+  long db_stride;
+  void *h;           /* optional: f(a) or f(a) * b from the checkpoints */
+  long h_stride;
+} ext_mpi_amd_act_grad;
+int ext_mpi_amd_act_grad_init(const ext_mpi_amd_act_grad *d, int *handle);
+
 /* ---- execution (stream-ordered on the handle's own HIP stream) ---- */
 int ext_mpi_amd_start(int handle);
 int ext_mpi_amd_test(int handle); /* 1 complete, 0 in flight, <0 error */

@@ -1,0 +1,114 @@
+"""The row operators without a GPU: refusals that come before any device is asked for, the test of two
+matrices for shared bytes, and the oracle's own checkpoint against the definition in 64 bits."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import ext_mpi_collectives_amd as emac
+import rows_ref as ref
+
+ARG, UNSUPPORTED = emac.ERROR_ARG, emac.ERROR_UNSUPPORTED
+
+
+def code_of(f, *a, **kw):
+    with pytest.raises(emac.ExtMpiError) as e:
+        f(*a, **kw)
+    return e.value.code
+
+
+CALLS = [
+    (lambda r, c, t: emac.layernorm_init(r, c, t, [64], 64)),
+    (lambda r, c, t: emac.layernorm_grad_init(r, c, t, [64], 64, 64, x=64, dx=64)),
+    (lambda r, c, t: emac.save8_init(r, c, t, 64, 64, 64)),
+    (lambda r, c, t: emac.restore8_init(r, c, t, 64, 64, 64)),
+    (lambda r, c, t: emac.act_init(r, c, t, emac.GELU, 64, 64)),
+    (lambda r, c, t: emac.act_grad_init(r, c, t, emac.GELU, 64, 64, 64, 64)),
+]
+
+
+@pytest.mark.parametrize("call", range(len(CALLS)))
+def test_refusals_before_the_device(call):
+    f = CALLS[call]
+    assert code_of(f, -1, 8, emac.FLOAT) == ARG
+    assert code_of(f, 1, 0, emac.FLOAT) == ARG
+    assert code_of(f, 1, -8, emac.FLOAT) == ARG
+    assert code_of(f, 1, 8, 6) == ARG and code_of(f, 1, 8, -1) == ARG
+    for t in (emac.DOUBLE, emac.LONG, emac.INT):
+        assert code_of(f, 1, 8, t) == UNSUPPORTED
+    assert code_of(f, 1, (1 << 30) + 1, emac.FLOAT) == UNSUPPORTED
+    if call < 2:
+        assert code_of(f, 1, emac.ROW_COLS_MAX + 1, emac.FLOAT) == UNSUPPORTED
+    if not torch.cuda.is_available():
+        assert code_of(f, 1, 8, emac.FLOAT) == emac.ERROR_DEVICE  # and no answer from the CPU
+
+
+def test_null_descriptors():
+    L, h = emac.lib(), ctypes.c_int(-1)
+    for name, desc in (("layernorm", emac.LayernormDesc), ("layernorm_grad", emac.LayernormGradDesc), ("act", emac.ActDesc),
+                       ("act_grad", emac.ActGradDesc)):
+        f = getattr(L, f"ext_mpi_amd_{name}_init")
+        assert f(None, ctypes.byref(h)) == ARG
+        assert f(ctypes.byref(desc()), None) == ARG
+    assert L.ext_mpi_amd_save8_init(1, 8, emac.FLOAT, None, 0, None, 0, None, None) == ARG
+    with pytest.raises(ValueError):
+        emac.layernorm_init(1, 8, emac.FLOAT, [], 64)
+    with pytest.raises(ValueError):
+        emac.layernorm_init(1, 8, emac.FLOAT, [64] * 17, 64)
+
+
+def test_the_allreduce_handles_refuse_the_new_types():
+    for t in (emac.BF16, emac.HALF):
+        assert code_of(emac.plan_describe, 2, 64, t, "6;1 -2 2", 0) == ARG
+
+
+def test_shared_bytes():
+    """Against the sets of bytes themselves."""
+    f = emac.lib().ext_mpi_amd_check_rows_share
+    f.argtypes = [ctypes.c_long] * 8
+    f.restype = ctypes.c_int
+    cells = lambda p, rows, ln, ld: {p + r * ld + k for r in range(rows) for k in range(ln)}  # noqa: E731
+    for rows_a in (1, 2, 5):
+        for rows_b in (1, 2, 5):
+            for len_a in (1, 3, 8):
+                for len_b in (1, 4, 8):
+                    for b in range(0, 70):
+                        a, ld = 20, 8
+                        shared = bool(cells(a, rows_a, len_a, ld) & cells(b, rows_b, len_b, ld))
+                        got = bool(f(a, rows_a, len_a, ld, b, rows_b, len_b, ld))
+                        assert got or not shared, (rows_a, rows_b, len_a, len_b, b)
+                        if rows_a == rows_b == 5 and len_a + len_b <= ld and not shared:
+                            assert not got, (len_a, len_b, b)  # interleaved rows are told apart
+    assert f(0, 4, 8, 16, 8, 4, 8, 32) == 1   # other strides that cross: refused
+    assert f(0, 4, 8, 16, 4096, 4, 8, 32) == 0
+
+
+def test_oracle_checkpoint():
+    """The oracle's bytes are the nearest of the definition's values, its scale within a rounding. Beyond the
+    half step a / 254: 127 / a and its product with x are off by U each of up to 127 steps, 2 U a; 1 / 127
+    and its product with a by U each, 2 U a; the restored product by U a."""
+    for t in ref.TYPES.values():
+        x = (torch.randn(7, 300, generator=torch.Generator().manual_seed(1)) * 3).to(t)
+        x[2], x[3, 5] = 0, 1000.0
+        q, s = ref.save8(x)
+        back = ref.restore8(q, s).double()
+        a = torch.zeros(7, 384).double()
+        a[:, :300] = x.double().abs()
+        a = a.view(7, 3, 128).amax(2)
+        assert bool(((s.double() * 127 - a).abs() <= 3 * ref.U * a + 2.0 ** -99).all())
+        lim = a.repeat_interleave(128, 1)[:, :300] * (1 / 254 + 5 * ref.U) + 2.0 ** -107
+        assert bool(((back - x.double()).abs() <= lim).all())
+        assert int(q.abs().max()) == 127 and not bool(q[2].any())
+    x = torch.ones(1, 256)
+    x[0, 3] = math.nan
+    q, s = ref.save8(x)
+    assert math.isnan(float(s[0, 0])) and not bool(q[0, :128].any()) and float(s[0, 1]) > 0
+
+
+def test_struct_layouts():
+    """The ctypes structures are the header's, byte for byte (8-byte pointers and longs, 4-byte ints)."""
+    assert ctypes.sizeof(emac.LayernormDesc) == 16 + 16 + 16 * 8 + 15 * 8
+    assert ctypes.sizeof(emac.LayernormGradDesc) == 16 + 24 + 16 * 8 + 18 * 8
+    assert ctypes.sizeof(emac.ActDesc) == 24 + 11 * 8
+    assert ctypes.sizeof(emac.ActGradDesc) == 24 + 13 * 8

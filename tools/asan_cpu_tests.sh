@@ -8,7 +8,7 @@ R=$(cd "$(dirname "$0")/.." && pwd)
 W=$(mktemp -d)
 B=$R/ext_mpi_collectives_amd/csrc/build
 make -s -C "$R/ext_mpi_collectives_amd/csrc" all
-ENG="engine engine_tune engine_node engine_comm engine_ipc engine_join"
+ENG="engine engine_rows engine_tune engine_node engine_comm engine_ipc engine_join"
 for f in plan layout $ENG; do
   gcc -O1 -g -fsanitize=address,undefined -fno-omit-frame-pointer -fPIC -std=gnu11 -D__HIP_PLATFORM_AMD__ \
     -I/opt/rocm/include -I"$R/include" -c "$R/ext_mpi_collectives_amd/csrc/$f.c" -o "$W/$f.o"
@@ -17,7 +17,7 @@ mkdir -p "$W/tree"
 (cd "$R" && git ls-files | tar -cf - -T -) | (cd "$W/tree" && tar -xf -)
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -fsanitize=address,undefined \
   -o "$W/tree/ext_mpi_collectives_amd/libext_mpi_amd.so" "$W"/plan.o "$W"/layout.o "$W"/engine*.o \
-  "$B"/ipc.o "$B"/fold*.o -L/opt/rocm/lib -lrccl \
+  "$B"/ipc.o "$B"/fold*.o "$B"/join_fused.o "$B"/norm*.o "$B"/act8.o "$B"/stamp.o -L/opt/rocm/lib -lrccl \
   -Wl,-rpath,/opt/rocm/lib
 make -s -C "$R/oracle"
 cp "$R/oracle/liboracle.so" "$W/tree/oracle/"
