@@ -2,7 +2,7 @@
 // checkpoints, and the checkpoints alone.
 //
 // Everything here is one pass over HBM: a 16-lane group owns one checkpoint block (128 columns of
-// one row), kUnroll groups' loads are issued before the first is used, and a block's maximum is a
+// one row), U groups' loads are issued before the first is used, and a block's maximum is a
 // reduction inside the group, so nothing is read twice and no barrier is needed. Blocks are
 // numbered row by row; a workgroup divides once (scalars) and a lane only where a row holds fewer
 // blocks than a workgroup takes. Bound by HBM; the arithmetic is about 30 lane operations per
@@ -13,7 +13,7 @@ namespace {
 
 using namespace emac_rows;
 
-constexpr int kUnroll = 4, kGroups = 16; // blocks a lane group takes, groups in a workgroup
+constexpr int kGroups = 16; // lane groups in a workgroup
 
 // ---- activations: value and slope, in 32 bits ----
 // 16-bit types take the native exp2 and reciprocal (1 ulp each); float the library's exp and IEEE
@@ -93,18 +93,19 @@ __device__ inline void act_both(float a, float &value, float &slope) {
   }
 }
 
-// where a lane's 8 elements of block `u` (0 .. kUnroll - 1) of its group lie
+// where a lane's 8 elements of block `u` (0 .. U - 1) of its group lie
 struct place {
   long row;
   int blk, c; // block of the row, first column of the lane
-  long n;     // elements from there to the row's end, 0 or less if none
+  int n;      // elements from there to the row's end, 0 or less if none
 };
+template <int U>
 struct span8 {
   long row0;
   unsigned blk0, nblk;
   long rows, cols;
   __device__ span8(long rows_, long cols_, unsigned nblk_) : nblk(nblk_), rows(rows_), cols(cols_) {
-    const unsigned first = blockIdx.x * (unsigned)(kUnroll * kGroups);
+    const unsigned first = blockIdx.x * (unsigned)(U * kGroups);
     row0 = first / nblk;
     blk0 = first - (unsigned)row0 * nblk;
   }
@@ -112,41 +113,41 @@ struct span8 {
     const unsigned x = blk0 + u * kGroups + threadIdx.x / 16;
     place p;
     unsigned k;
-    if (nblk >= (unsigned)(kUnroll * kGroups)) k = x >= nblk ? 1u : 0u;
+    if (nblk >= (unsigned)(U * kGroups)) k = x >= nblk ? 1u : 0u;
     else k = x / nblk;
     p.row = row0 + k;
     p.blk = (int)(x - k * nblk);
     p.c = p.blk * EMAC_BLOCK8 + (int)(threadIdx.x % 16) * 8;
-    p.n = p.row < rows ? cols - p.c : 0;
+    p.n = p.row < rows ? (int)cols - p.c : 0;
     return p;
   }
 };
 
 template <class T>
-__device__ inline void put8(const place &p, v8<T> x, signed char *q, long q_stride, float *scale, unsigned nblk) {
+__device__ inline void put8(const place &p, raw8<T> x, signed char *q, long q_stride, float *scale, unsigned nblk) {
   const block8 b = quantise<T>(x);
   if (p.n > 0) {
-    store8q(q + p.row * q_stride + p.c, b.q, p.n);
+    store8<signed char>(q + p.row * q_stride, p.c, b.q, p.n);
     if (threadIdx.x % 16 == 0) scale[p.row * nblk + p.blk] = b.scale;
   }
 }
 
-template <class T, int KIND, bool GATE>
+template <class T, int KIND, bool GATE, int U>
 __global__ __launch_bounds__(256) void act_kernel(const ext_mpi_amd_act d, unsigned nblk) {
-  const span8 s(d.rows, d.cols, nblk);
-  v8<T> a[kUnroll], b[GATE ? kUnroll : 1];
+  const span8<U> s(d.rows, d.cols, nblk);
+  raw8<T> a[U], b[GATE ? U : 1];
 #pragma unroll
-  for (int u = 0; u < kUnroll; u++) {
+  for (int u = 0; u < U; u++) {
     const place p = s.at(u);
-    a[u] = (v8<T>)(T)0;
+    a[u] = (raw8<T>)0u;
     if (GATE) b[GATE ? u : 0] = a[u];
     if (p.n > 0) {
-      a[u] = load8((const T *)d.a + p.row * d.a_stride + p.c, p.n);
-      if (GATE) b[GATE ? u : 0] = load8((const T *)d.b + p.row * d.b_stride + p.c, p.n);
+      a[u] = load8((const T *)d.a + p.row * d.a_stride, p.c, p.n);
+      if (GATE) b[GATE ? u : 0] = load8((const T *)d.b + p.row * d.b_stride, p.c, p.n);
     }
   }
 #pragma unroll
-  for (int u = 0; u < kUnroll; u++) {
+  for (int u = 0; u < U; u++) {
     const place p = s.at(u);
     if (d.qa) {
       put8<T>(p, a[u], d.qa, d.q_stride, d.sa, nblk);
@@ -159,33 +160,33 @@ __global__ __launch_bounds__(256) void act_kernel(const ext_mpi_amd_act d, unsig
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = act_value<T, KIND>(f[j]);
         if (GATE) v *= widen<T>(b[GATE ? u : 0]);
-        store8((T *)d.h + p.row * d.h_stride + p.c, round_to<T>(v), p.n);
+        store8<T>((T *)d.h + p.row * d.h_stride, p.c, round_to<T>(v), p.n);
       }
     }
   }
 }
 
-template <class T, int KIND, bool GATE>
+template <class T, int KIND, bool GATE, int U>
 __global__ __launch_bounds__(256) void act_grad_kernel(const ext_mpi_amd_act_grad d, unsigned nblk) {
-  const span8 s(d.rows, d.cols, nblk);
-  v8<T> g[kUnroll];
-  u2 qa[kUnroll], qb[GATE ? kUnroll : 1];
-  float sa[kUnroll], sb[GATE ? kUnroll : 1];
+  const span8<U> s(d.rows, d.cols, nblk);
+  raw8<T> g[U];
+  u2 qa[U], qb[GATE ? U : 1];
+  float sa[U], sb[GATE ? U : 1];
 #pragma unroll
-  for (int u = 0; u < kUnroll; u++) {
+  for (int u = 0; u < U; u++) {
     const place p = s.at(u);
     if (p.n > 0) {
-      g[u] = load8((const T *)d.dh + p.row * d.dh_stride + p.c, p.n);
-      qa[u] = load8q(d.qa + p.row * d.q_stride + p.c, p.n);
+      g[u] = load8((const T *)d.dh + p.row * d.dh_stride, p.c, p.n);
+      qa[u] = load8<signed char>(d.qa + p.row * d.q_stride, p.c, p.n);
       sa[u] = d.sa[p.row * nblk + p.blk];
       if (GATE) {
-        qb[GATE ? u : 0] = load8q(d.qb + p.row * d.q_stride + p.c, p.n);
+        qb[GATE ? u : 0] = load8<signed char>(d.qb + p.row * d.q_stride, p.c, p.n);
         sb[GATE ? u : 0] = d.sb[p.row * nblk + p.blk];
       }
     }
   }
 #pragma unroll
-  for (int u = 0; u < kUnroll; u++) {
+  for (int u = 0; u < U; u++) {
     const place p = s.at(u);
     if (p.n <= 0) continue;
     const f8 a = restore(qa[u], sa[u]), dh = widen<T>(g[u]);
@@ -200,34 +201,34 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const ext_mpi_amd_act_gra
     slope *= dh;
     if (GATE) {
       const f8 b = restore(qb[GATE ? u : 0], sb[GATE ? u : 0]);
-      store8((T *)d.da + p.row * d.da_stride + p.c, round_to<T>(slope * b), p.n);
-      store8((T *)d.db + p.row * d.db_stride + p.c, round_to<T>(dh * value), p.n);
+      store8<T>((T *)d.da + p.row * d.da_stride, p.c, round_to<T>(slope * b), p.n);
+      store8<T>((T *)d.db + p.row * d.db_stride, p.c, round_to<T>(dh * value), p.n);
       value *= b;
     } else {
-      store8((T *)d.da + p.row * d.da_stride + p.c, round_to<T>(slope), p.n);
+      store8<T>((T *)d.da + p.row * d.da_stride, p.c, round_to<T>(slope), p.n);
     }
-    if (d.h) store8((T *)d.h + p.row * d.h_stride + p.c, round_to<T>(value), p.n);
+    if (d.h) store8<T>((T *)d.h + p.row * d.h_stride, p.c, round_to<T>(value), p.n);
   }
 }
 
-template <class T>
+template <class T, int U>
 __global__ __launch_bounds__(256) void restore8_kernel(long rows, long cols, const signed char *q, long q_stride,
                                                        const float *scale, T *x, long x_stride, unsigned nblk) {
-  const span8 s(rows, cols, nblk);
-  u2 w[kUnroll];
-  float sc[kUnroll];
+  const span8<U> s(rows, cols, nblk);
+  u2 w[U];
+  float sc[U];
 #pragma unroll
-  for (int u = 0; u < kUnroll; u++) {
+  for (int u = 0; u < U; u++) {
     const place p = s.at(u);
     if (p.n > 0) {
-      w[u] = load8q(q + p.row * q_stride + p.c, p.n);
+      w[u] = load8<signed char>(q + p.row * q_stride, p.c, p.n);
       sc[u] = scale[p.row * nblk + p.blk];
     }
   }
 #pragma unroll
-  for (int u = 0; u < kUnroll; u++) {
+  for (int u = 0; u < U; u++) {
     const place p = s.at(u);
-    if (p.n > 0) store8(x + p.row * x_stride + p.c, round_to<T>(restore(w[u], sc[u])), p.n);
+    if (p.n > 0) store8<T>(x + p.row * x_stride, p.c, round_to<T>(restore(w[u], sc[u])), p.n);
   }
 }
 
@@ -235,52 +236,61 @@ __global__ __launch_bounds__(256) void restore8_kernel(long rows, long cols, con
 
 struct grid8 {
   unsigned nblk, grid;
+  int u;
 };
-// blocks and workgroups of a matrix (engine_rows.c holds rows * blocks under 2^31)
+// blocks, workgroups and blocks per lane group (engine_rows.c holds rows * blocks under 2^31): 4
+// blocks' loads in flight where that leaves 8 workgroups to a CU, else as many workgroups as can be
 grid8 grid_of(long rows, long cols) {
   grid8 g;
   g.nblk = (unsigned)((cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8);
-  g.grid = (unsigned)((rows * g.nblk + kUnroll * kGroups - 1) / (kUnroll * kGroups));
+  g.u = rows * g.nblk >= 4L * kGroups * 2048 ? 4 : 1;
+  g.grid = (unsigned)((rows * g.nblk + g.u * kGroups - 1) / (g.u * kGroups));
   return g;
 }
 
-template <class T, int KIND>
+template <class T, int KIND, bool GATE>
 int act_go(const ext_mpi_amd_act &d, hipStream_t st) {
   const grid8 g = grid_of(d.rows, d.cols);
-  if (d.b) act_kernel<T, KIND, true><<<g.grid, 256, 0, st>>>(d, g.nblk);
-  else act_kernel<T, KIND, false><<<g.grid, 256, 0, st>>>(d, g.nblk);
+  if (g.u == 4) act_kernel<T, KIND, GATE, 4><<<g.grid, 256, 0, st>>>(d, g.nblk);
+  else act_kernel<T, KIND, GATE, 1><<<g.grid, 256, 0, st>>>(d, g.nblk);
   return launched();
+}
+
+template <class T, int KIND>
+int act_k(const ext_mpi_amd_act &d, hipStream_t st) {
+  return d.b ? act_go<T, KIND, true>(d, st) : act_go<T, KIND, false>(d, st);
 }
 
 template <class T>
 int act_t(const ext_mpi_amd_act &d, hipStream_t st) {
   switch (d.kind) {
-  case EMAC_SAVE8: {
-    const grid8 g = grid_of(d.rows, d.cols);
-    act_kernel<T, EMAC_SAVE8, false><<<g.grid, 256, 0, st>>>(d, g.nblk);
-    return launched();
-  }
-  case EXT_MPI_AMD_SILU: return act_go<T, EXT_MPI_AMD_SILU>(d, st);
-  case EXT_MPI_AMD_GELU: return act_go<T, EXT_MPI_AMD_GELU>(d, st);
-  case EXT_MPI_AMD_GELU_TANH: return act_go<T, EXT_MPI_AMD_GELU_TANH>(d, st);
+  case EMAC_SAVE8: return act_go<T, EMAC_SAVE8, false>(d, st);
+  case EXT_MPI_AMD_SILU: return act_k<T, EXT_MPI_AMD_SILU>(d, st);
+  case EXT_MPI_AMD_GELU: return act_k<T, EXT_MPI_AMD_GELU>(d, st);
+  case EXT_MPI_AMD_GELU_TANH: return act_k<T, EXT_MPI_AMD_GELU_TANH>(d, st);
   }
   return EMAC_ERR_ARG;
 }
 
-template <class T, int KIND>
+template <class T, int KIND, bool GATE>
 int act_grad_go(const ext_mpi_amd_act_grad &d, hipStream_t st) {
   const grid8 g = grid_of(d.rows, d.cols);
-  if (d.qb) act_grad_kernel<T, KIND, true><<<g.grid, 256, 0, st>>>(d, g.nblk);
-  else act_grad_kernel<T, KIND, false><<<g.grid, 256, 0, st>>>(d, g.nblk);
+  if (g.u == 4) act_grad_kernel<T, KIND, GATE, 4><<<g.grid, 256, 0, st>>>(d, g.nblk);
+  else act_grad_kernel<T, KIND, GATE, 1><<<g.grid, 256, 0, st>>>(d, g.nblk);
   return launched();
+}
+
+template <class T, int KIND>
+int act_grad_k(const ext_mpi_amd_act_grad &d, hipStream_t st) {
+  return d.qb ? act_grad_go<T, KIND, true>(d, st) : act_grad_go<T, KIND, false>(d, st);
 }
 
 template <class T>
 int act_grad_t(const ext_mpi_amd_act_grad &d, hipStream_t st) {
   switch (d.kind) {
-  case EXT_MPI_AMD_SILU: return act_grad_go<T, EXT_MPI_AMD_SILU>(d, st);
-  case EXT_MPI_AMD_GELU: return act_grad_go<T, EXT_MPI_AMD_GELU>(d, st);
-  case EXT_MPI_AMD_GELU_TANH: return act_grad_go<T, EXT_MPI_AMD_GELU_TANH>(d, st);
+  case EXT_MPI_AMD_SILU: return act_grad_k<T, EXT_MPI_AMD_SILU>(d, st);
+  case EXT_MPI_AMD_GELU: return act_grad_k<T, EXT_MPI_AMD_GELU>(d, st);
+  case EXT_MPI_AMD_GELU_TANH: return act_grad_k<T, EXT_MPI_AMD_GELU_TANH>(d, st);
   }
   return EMAC_ERR_ARG;
 }
@@ -289,7 +299,8 @@ template <class T>
 int restore_t(long rows, long cols, const signed char *q, long q_stride, const float *scale, void *x, long x_stride,
               hipStream_t st) {
   const grid8 g = grid_of(rows, cols);
-  restore8_kernel<T><<<g.grid, 256, 0, st>>>(rows, cols, q, q_stride, scale, (T *)x, x_stride, g.nblk);
+  if (g.u == 4) restore8_kernel<T, 4><<<g.grid, 256, 0, st>>>(rows, cols, q, q_stride, scale, (T *)x, x_stride, g.nblk);
+  else restore8_kernel<T, 1><<<g.grid, 256, 0, st>>>(rows, cols, q, q_stride, scale, (T *)x, x_stride, g.nblk);
   return launched();
 }
 

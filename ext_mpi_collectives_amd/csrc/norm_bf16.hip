@@ -1,11 +1,7 @@
-// norm_bf16.hip -- bf16 instantiations of the layer norm kernels (one translation unit per element
-// type so that they compile in parallel). See norm_kernel.hpp.
+// norm_bf16.hip -- layer norm, bf16 rows and weights of the same type (one translation unit per
+// combination, so that they compile in parallel). See norm_kernel.hpp.
 #include "norm_kernel.hpp"
 
 extern "C" int emac_norm_launch_bf16(const ext_mpi_amd_layernorm *d, void *st) {
-  return emac_rows::norm_launch<emac_rows::bf16>(*d, static_cast<hipStream_t>(st));
-}
-
-extern "C" int emac_grad_launch_bf16(const ext_mpi_amd_layernorm_grad *d, float *part, void *st) {
-  return emac_rows::grad_launch<emac_rows::bf16>(*d, emac_rows::grad_shape_of(*d), part, static_cast<hipStream_t>(st));
+  return emac_rows::norm_w<emac_rows::bf16, emac_rows::bf16>(*d, static_cast<hipStream_t>(st));
 }

@@ -16,137 +16,223 @@
 
 namespace emac_rows {
 
-// the sum over a row's TPR lanes; `red` holds two slots per wave, used in turn (`turn` flips with
-// each call), so one barrier separates a slot's last read from its next write
-template <int TPR, int BLOCK, int NS>
+// How the lanes of a workgroup share out rows: MODE 16 or 64 lanes to a row, 256 lanes in all, or
+// (MODE 0) all of a workgroup of as many waves as the row needs at NV vectors to a lane, at most 8.
+// Few waves with many registers (up to 256) and the next row's loads in flight hide the latency; more
+// waves only repeat what every wave does once a row.
+template <int MODE>
+struct lanes {
+  static constexpr int kBlock = MODE ? 256 : 512; // at most
+  static constexpr int kWaves = MODE ? 4 : 2;     // waves to a SIMD that the registers allow
+  static constexpr int kRows = MODE ? 256 / MODE : 1;
+  int per, l, sub; // lanes to a row, this lane's place in it, its row in the workgroup
+  __device__ lanes() {
+    per = MODE ? MODE : (int)blockDim.x;
+    l = MODE ? threadIdx.x % (MODE ? MODE : 1) : threadIdx.x;
+    sub = MODE ? threadIdx.x / (MODE ? MODE : 1) : 0;
+    if (MODE == 64) sub = __builtin_amdgcn_readfirstlane(sub);
+  }
+};
+
+// A lane's vector i of a row. FULL (cols a multiple of 8): a vector lies inside the row or past it,
+// and a lane past it loads the row's last vector again, which is kept out of every sum and store --
+// no load has a branch. Else the last vector holds `n` elements and zeros.
+template <bool FULL>
+struct slot {
+  int c, n; // column, elements (0 or less: none)
+  __device__ slot(int i, int per, int l, int cols, bool live) {
+    const int at = (l + i * per) * 8;
+    n = live ? cols - at : 0;
+    c = FULL && at >= cols ? cols - 8 : at;
+  }
+  __device__ bool in() const { return n > 0; }
+  template <class T, bool again = false>
+  __device__ raw8<T> load(const void *row) const {
+    return load8<T, again>((const T *)row, (unsigned)c, FULL ? 8 : n);
+  }
+  template <class T>
+  __device__ void store(void *row, raw8<T> v) const {
+    if (in()) store8<T>((T *)row, (unsigned)c, v, FULL ? 8 : n);
+  }
+};
+template <class T>
+__device__ inline const T *row_of(const void *p, long row, long stride) {
+  return (const T *)p + row * stride;
+}
+
+// Sums over a row's lanes. Between waves they go through LDS: each wave leaves its own, and after
+// one barrier 8 lanes of every wave add the up to 8 of them; the two slots are used in turn, so
+// a slot's last read and its next write have a barrier between them.
+template <int MODE, int NS>
 struct row_sum {
-  static constexpr int kWaves = BLOCK / 64, kPer = TPR / 64;
-  __device__ static void run(float (&v)[NS], float (*red)[kWaves][NS], int &turn) {
-    if constexpr (TPR == 16) {
+  float (*red)[8][NS];
+  int turn;
+  __device__ row_sum(float (*r)[8][NS]) : red(r), turn(0) {
+    if (MODE == 0) { // the places of waves that are not there
+      const int nw = blockDim.x / 64, t = threadIdx.x;
+      if (t < 16 && t % 8 >= nw) {
 #pragma unroll
-      for (int k = 0; k < NS; k++) v[k] = sum16(v[k]);
-      return;
+        for (int k = 0; k < NS; k++) r[t / 8][t % 8][k] = 0.0f;
+      }
     }
+  }
+  __device__ void operator()(float (&v)[NS]) {
 #pragma unroll
-    for (int k = 0; k < NS; k++) v[k] = sum64(v[k]);
-    if constexpr (TPR > 64) {
-      const int wave = threadIdx.x / 64, first = wave / kPer * kPer;
+    for (int k = 0; k < NS; k++) v[k] = MODE == 16 ? sum16(v[k]) : sum64(v[k]);
+    if constexpr (MODE == 0) {
       if (threadIdx.x % 64 == 0) {
 #pragma unroll
-        for (int k = 0; k < NS; k++) red[turn][wave][k] = v[k];
+        for (int k = 0; k < NS; k++) red[turn][threadIdx.x / 64][k] = v[k];
       }
       __syncthreads();
 #pragma unroll
-      for (int k = 0; k < NS; k++) {
-        float s = red[turn][first][k];
-#pragma unroll
-        for (int w = 1; w < kPer; w++) s += red[turn][first + w][k];
-        v[k] = s;
-      }
+      for (int k = 0; k < NS; k++) v[k] = sum8(red[turn][threadIdx.x % 8][k]);
       turn ^= 1;
     }
   }
 };
 
-// ((leaf 0 + leaf 1) + ...) of 8 elements in 32 bits; four leaves' loads in flight at a time
-template <class T>
-__device__ inline f8 fold8(const void *const *src, int nsrc, long at, long n) {
+// ((leaf 0 + leaf 1) + ...) of 8 elements in 32 bits, the loads of a batch in flight together
+template <class T, bool FULL>
+__device__ inline f8 fold8(const void *const *src, int nsrc, long row, long stride, const slot<FULL> &at) {
+  constexpr int B = sizeof(T) == 2 ? 8 : 4;
   f8 s = {};
-  for (int t0 = 0; t0 < nsrc; t0 += 4) {
-    v8<T> raw[4];
+  for (int t0 = 0; t0 < nsrc; t0 += B) {
+    raw8<T> raw[B];
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-      if (t0 + k < nsrc) raw[k] = load8((const T *)src[t0 + k] + at, n);
+    for (int k = 0; k < B; k++)
+      if (t0 + k < nsrc) raw[k] = at.template load<T>(row_of<T>(src[t0 + k], row, stride));
 #pragma unroll
-    for (int k = 0; k < 4; k++)
+    for (int k = 0; k < B; k++)
       if (t0 + k < nsrc) s = t0 + k ? s + widen<T>(raw[k]) : widen<T>(raw[k]);
   }
   return s;
 }
 
-template <class T, class W, int NV, int TPR, int BLOCK, bool MULTI>
-__global__ __launch_bounds__(BLOCK) void layernorm_kernel(const ext_mpi_amd_layernorm d) {
-  constexpr int RPB = BLOCK / TPR;
-  __shared__ float red[2][BLOCK / 64][1];
-  int turn = 0;
-  const int l = threadIdx.x % TPR;
-  int sub = threadIdx.x / TPR;
-  if constexpr (TPR >= 64) sub = __builtin_amdgcn_readfirstlane(sub);
-  const int cols = (int)d.cols;
-  const int nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
-  for (long r0 = (long)blockIdx.x * RPB; r0 < d.rows; r0 += (long)gridDim.x * RPB) {
-    const long row = r0 + sub;
-    const bool live = row < d.rows;
-    v8<T> x[NV];
-    float s[1] = {0.0f};
+// A row's weights (`none` without any), in registers over all rows of a workgroup: as floats at up
+// to two vectors to a lane, else (AHEAD) as loaded. A load of them among the next row's would be worse
+// than its own latency: loads return in order, so waiting for it is waiting for the next row. Only the
+// forms that do not load ahead load them at their use. ZERO: zeros past the row's end.
+template <class W, int NV, bool FULL, bool ZERO, bool AHEAD>
+struct weights {
+  static constexpr bool kFloats = NV <= 2, kRaw = !kFloats && AHEAD;
+  f8 v[kFloats ? NV : 1];
+  raw8<W> r[kRaw ? NV : 1];
+  const W *p;
+  float none;
+  __device__ weights(const void *p_, float none_, int per, int l, int cols) : p((const W *)p_), none(none_) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const int c = (l + i * TPR) * 8;
-      const long n = live ? cols - c : 0;
-      if (n > 0) {
-        if (!MULTI && !d.residual) {
-          x[i] = load8((const T *)d.src[0] + row * d.src_stride + c, n);
-        } else {
-          f8 f;
-          v8<T> res;
-          if (d.residual) res = load8((const T *)d.residual + row * d.residual_stride + c, n);
-          if constexpr (MULTI)
-            f = fold8<T>(d.src, d.nsrc, row * d.src_stride + c, n);
-          else
-            f = widen<T>(load8((const T *)d.src[0] + row * d.src_stride + c, n));
-          if (d.residual) f += widen<T>(res);
-          x[i] = round_to<T>(f);
-        }
+      const slot<FULL> at(i, per, l, cols, true);
+      if (kFloats) v[kFloats ? i : 0] = floats(p ? at.template load<W, true>(p) : (raw8<W>)0u, at);
+      if (kRaw && p) r[kRaw ? i : 0] = at.template load<W, true>(p);
+    }
+  }
+  __device__ f8 floats(raw8<W> w, const slot<FULL> &at) const {
+    f8 f = p ? widen<W>(w) : (f8)none;
+    if (ZERO && !at.in()) f = (f8)0.0f;
+    return f;
+  }
+  __device__ f8 at(int i, const slot<FULL> &s) const {
+    if (kFloats) return v[kFloats ? i : 0];
+    raw8<W> w = (raw8<W>)0u;
+    if (kRaw) {
+      w = r[kRaw ? i : 0];
+      hold(w); // widened at each use: the floats would stay in twice the registers
+    } else if (p) {
+      w = s.template load<W, true>(p);
+    }
+    return floats(w, s);
+  }
+};
+
+template <class T, class W, int MODE, int NV, bool MULTI, bool FULL>
+__global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void layernorm_kernel(const ext_mpi_amd_layernorm d) {
+  constexpr bool AHEAD = !MULTI && NV * sizeof(T) <= 8; // the next row's loads are issued before this row's sums
+  const lanes<MODE> ln;
+  const int l = ln.l, per = ln.per, cols = (int)d.cols;
+  const int nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
+  const float inv = 1.0f / (float)cols;
+  __shared__ float red[2][8][1];
+  row_sum<MODE, 1> sum_row(red);
+  const weights<W, NV, FULL, false, AHEAD> w(d.weight, 1.0f, per, l, cols), b(d.bias, 0.0f, per, l, cols);
+  const long step = (long)gridDim.x * ln.kRows;
+  raw8<T> nx[MULTI ? 1 : NV], nr[NV];
+  const auto load = [&](long row) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const slot<FULL> at(i, per, l, cols, true);
+      if (!MULTI) nx[MULTI ? 0 : i] = at.template load<T>(row_of<T>(d.src[0], row, d.src_stride));
+      if (d.residual) nr[i] = at.template load<T>(row_of<T>(d.residual, row, d.residual_stride));
+    }
+  };
+  // past the last row the last one is loaded again: no branch around the loads
+  const auto within = [&](long row) { return row < d.rows ? row : d.rows - 1; };
+  long r0 = (long)blockIdx.x * ln.kRows;
+  if (AHEAD) load(within(r0 + ln.sub));
+  for (; r0 < d.rows; r0 += step) {
+    const long row = r0 + ln.sub;
+    const bool live = MODE == 0 || row < d.rows;
+    raw8<T> x[NV];
+    float s[1] = {0.0f};
+    if (!AHEAD) load(within(row));
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const slot<FULL> at(i, per, l, cols, true);
+      if (MULTI || d.residual) {
+        f8 f;
+        if (MULTI) f = fold8<T>(d.src, d.nsrc, within(row), d.src_stride, at);
+        else f = widen<T>(nx[MULTI ? 0 : i]);
+        if (d.residual) f += widen<T>(nr[i]);
+        x[i] = round_to<T>(f);
       } else {
-        x[i] = (v8<T>)(T)0;
+        x[i] = nx[MULTI ? 0 : i];
       }
+      if (FULL && !at.in()) x[i] = (raw8<T>)0u;
+    }
+    if (AHEAD) load(within(row + step));
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
       const f8 f = widen<T>(x[i]);
 #pragma unroll
       for (int j = 0; j < 8; j++) s[0] += f[j];
     }
+    if (d.y || d.mean || d.rstd) {
+      sum_row(s);
+      const float mean = s[0] * inv;
+      s[0] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        const slot<FULL> at(i, per, l, cols, true);
+        const f8 f = widen<T>(x[i]) - mean;
+        float t = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) t += FULL || j < at.n ? f[j] * f[j] : 0.0f;
+        s[0] += at.in() ? t : 0.0f;
+      }
+      sum_row(s);
+      const float rstd = 1.0f / sqrtf(s[0] * inv + (float)d.eps);
+      if (l == 0 && live) {
+        if (d.mean) d.mean[row] = mean;
+        if (d.rstd) d.rstd[row] = rstd;
+      }
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        const slot<FULL> at(i, per, l, cols, live);
+        if (!d.y) continue;
+        const f8 f = (widen<T>(x[i]) - mean) * rstd * w.at(i, at) + b.at(i, at);
+        at.template store<T>((T *)d.y + row * d.y_stride, round_to<T>(f));
+      }
+    }
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const int c = (l + i * TPR) * 8;
-      const long n = live ? cols - c : 0;
-      if (d.sum && n > 0) store8((T *)d.sum + row * d.sum_stride + c, x[i], n);
+      const slot<FULL> at(i, per, l, cols, live);
+      if (d.sum) at.template store<T>((T *)d.sum + row * d.sum_stride, x[i]);
       if (d.q) { // every lane of a block takes part; lanes past the row hold zeros
-        const block8 b = quantise<T>(x[i]);
-        if (n > 0) {
-          store8q(d.q + row * d.q_stride + c, b.q, n);
-          if (c % EMAC_BLOCK8 == 0) d.scale[row * nblk + c / EMAC_BLOCK8] = b.scale;
-        }
+        const block8 k = quantise<T>(x[i]);
+        at.template store<signed char>(d.q + row * d.q_stride, k.q);
+        if (at.in() && at.c % EMAC_BLOCK8 == 0) d.scale[row * nblk + at.c / EMAC_BLOCK8] = k.scale;
       }
-    }
-    if (!d.y && !d.mean && !d.rstd) continue;
-    row_sum<TPR, BLOCK, 1>::run(s, red, turn);
-    const float mean = s[0] / (float)cols;
-    s[0] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const int c = (l + i * TPR) * 8, n = cols - c;
-      const f8 f = widen<T>(x[i]);
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float t = f[j] - mean;
-        s[0] += j < n ? t * t : 0.0f;
-      }
-    }
-    row_sum<TPR, BLOCK, 1>::run(s, red, turn);
-    const float rstd = 1.0f / sqrtf(s[0] / (float)cols + (float)d.eps);
-    if (l == 0 && live) {
-      if (d.mean) d.mean[row] = mean;
-      if (d.rstd) d.rstd[row] = rstd;
-    }
-    if (!d.y) continue;
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const int c = (l + i * TPR) * 8;
-      const long n = live ? cols - c : 0;
-      if (n <= 0) continue;
-      f8 f = (widen<T>(x[i]) - mean) * rstd;
-      if (d.weight) f *= widen<W>(load8((const W *)d.weight + c, n));
-      if (d.bias) f += widen<W>(load8((const W *)d.bias + c, n));
-      store8((T *)d.y + row * d.y_stride + c, round_to<T>(f), n);
     }
   }
 }
@@ -165,14 +251,15 @@ __device__ inline void put_grad(void *out, int gdtype, int accumulate, long c, f
   }
 }
 
-// a workgroup's column sums of 8 columns: into its partial row, or (one workgroup) the gradients
-__device__ inline void put_cols(const ext_mpi_amd_layernorm_grad &d, float *part, int c, f8 w, f8 b) {
+// Column sums that a workgroup has finished, 8 of each at column c, into its partial row, or (no
+// partial rows) into the gradients
+__device__ inline void put_cols(const ext_mpi_amd_layernorm_grad &d, float *part, int slice, int c, f8 w, f8 b) {
   const int cols = (int)d.cols, n = cols - c;
   if (n <= 0) return;
   if (part) {
-    float *p = part + (long)blockIdx.x * 2 * cols;
-    store8(p + c, w, n);
-    store8(p + cols + c, b, n);
+    float *p = part + (long)slice * 2 * cols;
+    store8<float, true>(p, c, round_to<float>(w), n);
+    store8<float, true>(p + cols, c, round_to<float>(b), n);
     return;
   }
 #pragma unroll
@@ -183,250 +270,335 @@ __device__ inline void put_cols(const ext_mpi_amd_layernorm_grad &d, float *part
     }
 }
 
-// xh = (x - mean) * rstd of 8 elements, from x or its checkpoint
-template <class T, bool Q8>
-__device__ inline f8 load_x(const ext_mpi_amd_layernorm_grad &d, long row, int c, long n, int nblk) {
-  if constexpr (Q8)
-    return restore(load8q(d.q + row * d.q_stride + c, n), d.scale[row * nblk + c / EMAC_BLOCK8]);
-  else
-    return widen<T>(load8((const T *)d.x + row * d.x_stride + c, n));
-}
-template <class T, bool MULTI>
-__device__ inline f8 load_g(const ext_mpi_amd_layernorm_grad &d, long row, int c, long n) {
-  if constexpr (MULTI)
-    return fold8<T>(d.dy, d.nsrc, row * d.dy_stride + c, n);
-  else
-    return widen<T>(load8((const T *)d.dy[0] + row * d.dy_stride + c, n));
-}
+// x of a row, or its checkpoint, as loaded
+template <class T, bool Q8, bool FULL>
+struct row8 {
+  raw8<T> x;
+  u2 q;
+  float scale;
+  __device__ void load(const ext_mpi_amd_layernorm_grad &d, long row, const slot<FULL> &at, int nblk) {
+    if (Q8) {
+      q = at.template load<signed char>(d.q + row * d.q_stride);
+      scale = d.scale[row * nblk + min(at.c / EMAC_BLOCK8, nblk - 1)];
+    } else {
+      x = at.template load<T>(row_of<T>(d.x, row, d.x_stride));
+    }
+  }
+  // (x - mean) * rstd, as x * rstd - mean * rstd: two roundings of the products' size
+  __device__ f8 normed(float rstd, float shift) const {
+    if constexpr (Q8) {
+      const float s = scale * rstd;
+      return bytes(q) * s + shift;
+    } else {
+      return widen<T>(x) * rstd + shift;
+    }
+  }
+};
 
-template <class T, class W, int NV, int TPR, int BLOCK, bool Q8, bool MULTI, bool ACC>
-__global__ __launch_bounds__(BLOCK) void layernorm_grad_kernel(const ext_mpi_amd_layernorm_grad d, float *part) {
-  constexpr int RPB = BLOCK / TPR;
-  __shared__ float red[2][BLOCK / 64][2];
-  int turn = 0;
-  const int l = threadIdx.x % TPR;
-  int sub = threadIdx.x / TPR;
-  if constexpr (TPR >= 64) sub = __builtin_amdgcn_readfirstlane(sub);
-  const int cols = (int)d.cols;
+// The rows of workgroup `block` of `blocks`: dx, y, and with ACC the two column sums.
+template <class T, class W, int MODE, int NV, bool Q8, bool MULTI, bool FULL, bool ACC>
+__device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block, int blocks, float *part) {
+  // one leaf: the next row's loads are issued before this row's sums, as far as registers go
+  constexpr bool AHEAD = !MULTI && NV <= 2;
+  // y has kernels of its own (the ones for any number of leaves and any width): a load of the bias
+  // among the next row's, even where no y is asked for, makes every row wait for the next
+  constexpr bool Y = MULTI && !FULL;
+  const lanes<MODE> ln;
+  const int l = ln.l, per = ln.per, cols = (int)d.cols;
   const int nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
+  const float inv = 1.0f / (float)cols;
+  __shared__ float red[2][8][2];
+  row_sum<MODE, 2> sum_row(red);
+  // zeros past the row's end: what a lane there loads enters no sum of the row
+  const weights<W, NV, FULL, true, AHEAD> w(d.weight, 1.0f, per, l, cols);
+  const long step = (long)blocks * ln.kRows;
+  const bool more = d.dsum && d.dx;
   f8 aw[ACC ? NV : 1] = {}, ab[ACC ? NV : 1] = {};
-  for (long r0 = (long)blockIdx.x * RPB; r0 < d.rows; r0 += (long)gridDim.x * RPB) {
-    const long row = r0 + sub;
-    const bool live = row < d.rows;
-    const float mean = live ? d.mean[row] : 0.0f, rstd = live ? d.rstd[row] : 0.0f;
-    f8 g[NV], xh[NV]; // g w after the sums
+  raw8<T> ng[MULTI ? 1 : NV], nd[NV];
+  row8<T, Q8, FULL> nx[NV];
+  float nmean, nrstd;
+  const auto load = [&](long row) {
+    nmean = d.mean[row];
+    nrstd = d.rstd[row];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const slot<FULL> at(i, per, l, cols, true);
+      if (!MULTI) ng[MULTI ? 0 : i] = at.template load<T>(row_of<T>(d.dy[0], row, d.dy_stride));
+      nx[i].load(d, row, at, nblk);
+      if (more) nd[i] = at.template load<T>(row_of<T>(d.dsum, row, d.dsum_stride));
+    }
+  };
+  const auto within = [&](long row) { return row < d.rows ? row : d.rows - 1; };
+  long r0 = (long)block * ln.kRows;
+  if (AHEAD) load(within(r0 + ln.sub));
+  for (; r0 < d.rows; r0 += step) {
+    const long row = r0 + ln.sub;
+    const bool live = MODE == 0 || row < d.rows;
+    if (!AHEAD) load(within(row));
+    const float rstd = nrstd, shift = -nmean * rstd;
+    f8 g[NV], xh[NV];
+    raw8<T> dsum[NV];
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const int c = (l + i * TPR) * 8;
-      const long n = live ? cols - c : 0;
-      if (n > 0) {
-        g[i] = load_g<T, MULTI>(d, row, c, n);
-        xh[i] = (load_x<T, Q8>(d, row, c, n, nblk) - mean) * rstd;
-      } else {
-        g[i] = xh[i] = (f8)0.0f;
-      }
+      const slot<FULL> at(i, per, l, cols, true);
+      if (MULTI) g[i] = fold8<T>(d.dy, d.nsrc, within(row), d.dy_stride, at);
+      else g[i] = widen<T>(ng[MULTI ? 0 : i]);
+      if (MODE != 0 && !live) g[i] = (f8)0.0f; // a row past the last
+      xh[i] = nx[i].normed(rstd, shift);
+      dsum[i] = nd[i];
     }
+    if (AHEAD) load(within(row + step));
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const int c = (l + i * TPR) * 8;
-      const long n = live ? cols - c : 0;
-      if (n <= 0) continue;
+      const slot<FULL> at(i, per, l, cols, live);
+      const f8 ww = w.at(i, at);
       if (ACC) {
         aw[ACC ? i : 0] += g[i] * xh[i];
         ab[ACC ? i : 0] += g[i];
       }
-      f8 w = (f8)1.0f;
-      if (d.weight) w = widen<W>(load8((const W *)d.weight + c, n));
-      if (d.y) {
-        f8 y = xh[i] * w;
-        if (d.bias) y += widen<W>(load8((const W *)d.bias + c, n));
-        store8((T *)d.y + row * d.y_stride + c, round_to<T>(y), n);
+      if (Y && d.y) {
+        f8 y = xh[i] * ww;
+        if (d.bias) y += widen<W>(at.template load<W, true>(d.bias));
+        at.template store<T>((T *)d.y + row * d.y_stride, round_to<T>(y));
       }
-      g[i] *= w;
+      g[i] *= ww;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        s[0] += j < n ? g[i][j] : 0.0f;
-        s[1] += j < n ? g[i][j] * xh[i][j] : 0.0f;
+        s[0] += g[i][j];
+        s[1] += g[i][j] * xh[i][j];
       }
     }
     if (!d.dx) continue;
-    row_sum<TPR, BLOCK, 2>::run(s, red, turn);
-    const float c1 = s[0] / (float)cols, c2 = s[1] / (float)cols;
+    sum_row(s);
+    const float c1 = -s[0] * inv * rstd, c2 = -s[1] * inv * rstd;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const int c = (l + i * TPR) * 8;
-      const long n = live ? cols - c : 0;
-      if (n <= 0) continue;
-      f8 dx = rstd * (g[i] - c1 - xh[i] * c2);
-      if (d.dsum) dx += widen<T>(load8((const T *)d.dsum + row * d.dsum_stride + c, n));
-      store8((T *)d.dx + row * d.dx_stride + c, round_to<T>(dx), n);
+      const slot<FULL> at(i, per, l, cols, live);
+      f8 dx = xh[i] * c2 + c1;
+      dx += g[i] * rstd;
+      if (more) dx += widen<T>(dsum[i]);
+      at.template store<T>((T *)d.dx + row * d.dx_stride, round_to<T>(dx));
     }
   }
   if constexpr (ACC) {
     if (!d.dweight && !d.dbias) return;
-    if constexpr (RPB > 1) { // the rows of a workgroup taken side by side, added in order
-      __shared__ f8 comb[2][TPR * NV];
-      for (int k = 1; k < RPB; k++) {
+    if constexpr (MODE != 0) { // the rows of a workgroup taken side by side, added in order
+      __shared__ f8 comb[2][(MODE ? MODE : 1) * NV];
+      for (int k = 1; k < ln.kRows; k++) {
         __syncthreads();
-        if (sub == k) {
+        if (ln.sub == k) {
 #pragma unroll
           for (int i = 0; i < NV; i++) {
-            comb[0][l + i * TPR] = aw[i];
-            comb[1][l + i * TPR] = ab[i];
+            comb[0][l + i * per] = aw[i];
+            comb[1][l + i * per] = ab[i];
           }
         }
         __syncthreads();
-        if (sub == 0) {
+        if (ln.sub == 0) {
 #pragma unroll
           for (int i = 0; i < NV; i++) {
-            aw[i] += comb[0][l + i * TPR];
-            ab[i] += comb[1][l + i * TPR];
+            aw[i] += comb[0][l + i * per];
+            ab[i] += comb[1][l + i * per];
           }
         }
       }
-      if (sub) return;
+      if (ln.sub) return;
     }
 #pragma unroll
-    for (int i = 0; i < NV; i++) put_cols(d, part, (l + i * TPR) * 8, aw[i], ab[i]);
+    for (int i = 0; i < NV; i++) put_cols(d, part, block, (l + i * per) * 8, aw[i], ab[i]);
   }
 }
 
-// The column sums alone, for rows too wide to keep them in registers beside the row: a wave takes
-// 512 columns of every fourth of its slice's rows. grid: slices (x), column tiles (y).
-template <class T, bool Q8, bool MULTI>
-__global__ __launch_bounds__(256) void layernorm_cols_kernel(const ext_mpi_amd_layernorm_grad d, float *part) {
-  __shared__ f8 comb[2][4][64];
-  const int l = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const int cols = (int)d.cols, c = ((int)blockIdx.y * 64 + l) * 8;
-  const int nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
+template <class T, class W, int MODE, int NV, bool Q8, bool MULTI, bool FULL>
+__global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void layernorm_grad_kernel(
+    const ext_mpi_amd_layernorm_grad d, float *part) {
+  grad_rows<T, W, MODE, NV, Q8, MULTI, FULL, true>(d, blockIdx.x, gridDim.x, part);
+}
+
+// The column sums alone: a workgroup takes 8 * LANES columns of every slices'th group of rows, as
+// many rows at a time as it has lanes for. `part` as in put_cols.
+template <class T, int LANES, bool Q8, bool MULTI, bool FULL>
+__device__ inline void cols_tile(const ext_mpi_amd_layernorm_grad &d, int tile, int slice, int slices, float *part) {
+  constexpr int C = 8 * LANES;
+  __shared__ float comb[2][512 / LANES][C];
+  const int l = threadIdx.x % LANES, k0 = threadIdx.x / LANES, R = blockDim.x / LANES;
+  const int cols = (int)d.cols, nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
+  const slot<FULL> at(0, 0, tile * LANES + l, cols, true);
   f8 aw = {}, ab = {};
-  if (c < cols)
-    for (long row = (long)blockIdx.x * 4 + wave; row < d.rows; row += (long)gridDim.x * 4) {
-      const f8 g = load_g<T, MULTI>(d, row, c, cols - c);
-      const f8 xh = (load_x<T, Q8>(d, row, c, cols - c, nblk) - d.mean[row]) * d.rstd[row];
-      aw += g * xh;
-      ab += g;
-    }
-  comb[0][wave][l] = aw;
-  comb[1][wave][l] = ab;
-  __syncthreads();
-  if (wave) return;
-  for (int k = 1; k < 4; k++) {
-    aw += comb[0][k][l];
-    ab += comb[1][k][l];
+#pragma unroll 4
+  for (long row = (long)slice * R + k0; row < d.rows; row += (long)slices * R) {
+    row8<T, Q8, FULL> x;
+    x.load(d, row, at, nblk);
+    const float rstd = d.rstd[row], mean = d.mean[row];
+    f8 g;
+    if (MULTI) g = fold8<T>(d.dy, d.nsrc, row, d.dy_stride, at);
+    else g = widen<T>(at.template load<T>(row_of<T>(d.dy[0], row, d.dy_stride)));
+    aw += g * x.normed(rstd, -mean * rstd);
+    ab += g;
   }
-  put_cols(d, part, c, aw, ab);
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    comb[0][k0][8 * l + j] = aw[j];
+    comb[1][k0][8 * l + j] = ab[j];
+  }
+  __syncthreads();
+  for (int o = threadIdx.x; o < 2 * C; o += blockDim.x) {
+    const int which = o / C, c = o % C, col = tile * C + c;
+    if (col >= cols) continue;
+    float s = 0.0f;
+    for (int k = 0; k < R; k++) s += comb[which][k][c];
+    void *out = which ? d.dbias : d.dweight;
+    if (part) part[(long)slice * 2 * cols + (long)which * cols + col] = s;
+    else if (out) put_grad(out, d.gdtype, d.accumulate, col, s);
+  }
+}
+
+// For rows too wide to keep the sums in registers beside the row: a wave takes 512 columns.
+// grid: slices (x), column tiles (y).
+template <class T, bool Q8>
+__global__ __launch_bounds__(256) void layernorm_cols_kernel(const ext_mpi_amd_layernorm_grad d, float *part) {
+  cols_tile<T, 64, Q8, true, false>(d, blockIdx.y, blockIdx.x, gridDim.x, part);
+}
+
+// Rows without column sums, and in the workgroups behind theirs (from `blocks` on) the column sums of
+// 64 columns each over all rows: the rows are read twice, but nothing waits for anything.
+template <class T, class W, int MODE, int NV, bool Q8>
+__global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void layernorm_grad_apart_kernel(
+    const ext_mpi_amd_layernorm_grad d, int blocks) {
+  if ((int)blockIdx.x < blocks) grad_rows<T, W, MODE, NV, Q8, true, false, false>(d, blockIdx.x, blocks, nullptr);
+  else if (d.nsrc == 1 && d.cols % 8 == 0) cols_tile<T, 8, Q8, false, true>(d, blockIdx.x - blocks, 0, 1, nullptr);
+  else cols_tile<T, 8, Q8, true, false>(d, blockIdx.x - blocks, 0, 1, nullptr);
 }
 
 // ---- launches ----
 
 #define EMAC_NORM_CUS 256 // compute units of the part
 
-template <class T, class W, int NV, int TPR, int BLOCK>
-int norm_go(const ext_mpi_amd_layernorm &d, hipStream_t st) {
-  const long want = (d.rows + BLOCK / TPR - 1) / (BLOCK / TPR), most = 2048L * EMAC_NORM_CUS / BLOCK * 2;
+// The launch of a norm of `cols` columns: lanes to a row, vectors to a lane, lanes of a workgroup.
+struct row_shape {
+  int mode, nv, block;
+};
+inline row_shape row_shape_of(long cols) {
+  const long v = (cols + 7) / 8; // vectors in a row
+  row_shape s;
+  s.mode = v <= 16 ? 16 : v <= 64 ? 64 : 0;
+  s.nv = s.mode || v <= 512 ? 1 : v <= 1024 ? 2 : v <= 2048 ? 4 : v <= 4096 ? 8 : 16;
+  s.block = s.mode ? 256 : (int)((v + s.nv - 1) / s.nv + 63) / 64 * 64;
+  return s;
+}
+
+template <class T, class W, int MODE, int NV, bool MULTI, bool FULL>
+int norm_go(const ext_mpi_amd_layernorm &d, const row_shape &s, hipStream_t st) {
+  constexpr int rows = lanes<MODE>::kRows;
+  const long want = (d.rows + rows - 1) / rows;
+  const long most = (long)EMAC_NORM_CUS * ((512 + s.block - 1) / s.block); // 8 waves to a CU, or a few more
   const int grid = (int)(want < most ? want : most);
-  if (d.nsrc > 1)
-    layernorm_kernel<T, W, NV, TPR, BLOCK, true><<<grid, BLOCK, 0, st>>>(d);
-  else
-    layernorm_kernel<T, W, NV, TPR, BLOCK, false><<<grid, BLOCK, 0, st>>>(d);
+  layernorm_kernel<T, W, MODE, NV, MULTI, FULL><<<grid, s.block, 0, st>>>(d);
   return launched();
+}
+
+template <class T, class W, int MODE, int NV>
+int norm_nv(const ext_mpi_amd_layernorm &d, const row_shape &s, hipStream_t st) {
+  const bool full = d.cols % 8 == 0;
+  if (d.nsrc > 1) return full ? norm_go<T, W, MODE, NV, true, true>(d, s, st) : norm_go<T, W, MODE, NV, true, false>(d, s, st);
+  return full ? norm_go<T, W, MODE, NV, false, true>(d, s, st) : norm_go<T, W, MODE, NV, false, false>(d, s, st);
 }
 
 template <class T, class W>
 int norm_w(const ext_mpi_amd_layernorm &d, hipStream_t st) {
-  const long v = (d.cols + 7) / 8; // vectors in a row
-  const bool few = d.rows < 2 * EMAC_NORM_CUS;
-  if (v <= 16) return norm_go<T, W, 1, 16, 256>(d, st);
-  if (v <= 64) return norm_go<T, W, 1, 64, 256>(d, st);
-  if (v <= 128 && !few) return norm_go<T, W, 2, 64, 256>(d, st);
-  if (v <= 256) return norm_go<T, W, 1, 256, 256>(d, st);
-  if (v <= 512 && !few) return norm_go<T, W, 2, 256, 256>(d, st);
-  if (v <= 1024 && !few) return norm_go<T, W, 4, 256, 256>(d, st);
-  if (v <= 1024) return norm_go<T, W, 1, 1024, 1024>(d, st);
-  if (v <= 2048) return norm_go<T, W, 2, 1024, 1024>(d, st);
-  if (v <= 4096) return norm_go<T, W, 4, 1024, 1024>(d, st);
-  return norm_go<T, W, 8, 1024, 1024>(d, st);
+  const row_shape s = row_shape_of(d.cols);
+  if (s.mode == 16) return norm_nv<T, W, 16, 1>(d, s, st);
+  if (s.mode == 64) return norm_nv<T, W, 64, 1>(d, s, st);
+  if (s.nv == 1) return norm_nv<T, W, 0, 1>(d, s, st);
+  if (s.nv == 2) return norm_nv<T, W, 0, 2>(d, s, st);
+  if (s.nv == 4) return norm_nv<T, W, 0, 4>(d, s, st);
+  // wider: the forms that take any number of leaves and any width
+  if (s.nv == 8) return norm_go<T, W, 0, 8, true, false>(d, s, st);
+  return norm_go<T, W, 0, 16, true, false>(d, s, st);
 }
 
-template <class T>
-int norm_launch(const ext_mpi_amd_layernorm &d, hipStream_t st) {
-  if (d.wdtype == d.dtype || !(d.weight || d.bias)) return norm_w<T, T>(d, st);
-  return norm_w<T, float>(d, st);
-}
-
-// workgroups of the gradient, each of which leaves one partial row
+// the gradient's launch: `grid` workgroups take the rows, and each leaves a partial row of column
+// sums; or (apart) `tiles` more take the column sums, in a launch before the rows' where dx replaces
+// what they read (the same sums either way)
 struct grad_shape {
-  int tpr, nv, block, grid;
-  bool wide;
+  row_shape r;
+  int grid, tiles;
+  bool apart, before;
+  bool wide; // two column sums beside a row's values no longer fit in registers
 };
 inline grad_shape grad_shape_of(const ext_mpi_amd_layernorm_grad &d) {
-  const long v = (d.cols + 7) / 8;
-  grad_shape s = {1024, 2, 1024, 0, false};
-  if (v <= 16) s = {16, 1, 256, 0, false};
-  else if (v <= 64) s = {64, 1, 256, 0, false};
-  else if (v <= 128) s = {64, 2, 256, 0, false};
-  else if (v <= 256) s = {256, 1, 256, 0, false};
-  else if (v <= 512) s = {512, 1, 512, 0, false};
-  else if (v <= 1024) s = {1024, 1, 1024, 0, false};
-  else if (v > 2048) s = {1024, v <= 4096 ? 4 : 8, 1024, 0, true};
-  const long want = (d.rows + s.block / s.tpr - 1) / (s.block / s.tpr), most = 1024L * EMAC_NORM_CUS / s.block;
+  grad_shape s;
+  s.r = row_shape_of(d.cols);
+  s.wide = s.r.nv > 4;
+  const bool sums = d.dweight || d.dbias;
+  const long rows = s.r.mode ? 256 / s.r.mode : 1, want = (d.rows + rows - 1) / rows;
+  // few rows: the second launch, which adds the partial rows, costs more than reading the rows twice,
+  // up to 4 of them to a lane (bf16, 4096 columns: 32 rows 4.5 us against 6.3, 256 rows 7.0 against
+  // 10.7, 512 rows, 8 to a lane, 12.0 against 11.1)
+  s.before = d.dx && d.dx == d.x;
+  for (int i = 0; i < d.nsrc; i++) s.before = s.before || (d.dx && d.dx == d.dy[i]);
+  const long twice = d.rows * d.cols * (d.nsrc + 1) * (d.dtype == EXT_MPI_AMD_FLOAT ? 4 : 2);
+  const int lanes = s.r.block < 256 ? 256 : s.r.block; // more rows at a time for the column sums
+  s.apart = sums && d.rows <= 4 * (lanes / 8) && twice <= 16L << 20;
+  s.tiles = s.apart ? (int)((d.cols + 63) / 64) : 0;
+  if (s.apart) s.r.block = lanes;
+  const long most = s.apart ? 2048 : (long)EMAC_NORM_CUS * (s.r.block > 256 ? 1 : 512 / s.r.block); // 8 waves to a CU, or a few fewer
   s.grid = (int)(want < most ? want : most);
+  if (s.apart && !d.dx && !d.y) s.grid = 0;
   return s;
 }
 
-template <class T, class W, int NV, int TPR, int BLOCK, bool ACC>
-int grad_go(const ext_mpi_amd_layernorm_grad &d, int grid, float *part, hipStream_t st) {
-  if (d.q && d.nsrc > 1)
-    layernorm_grad_kernel<T, W, NV, TPR, BLOCK, true, true, ACC><<<grid, BLOCK, 0, st>>>(d, part);
-  else if (d.q)
-    layernorm_grad_kernel<T, W, NV, TPR, BLOCK, true, false, ACC><<<grid, BLOCK, 0, st>>>(d, part);
-  else if (d.nsrc > 1)
-    layernorm_grad_kernel<T, W, NV, TPR, BLOCK, false, true, ACC><<<grid, BLOCK, 0, st>>>(d, part);
-  else
-    layernorm_grad_kernel<T, W, NV, TPR, BLOCK, false, false, ACC><<<grid, BLOCK, 0, st>>>(d, part);
+template <class T, class W, int MODE, int NV>
+int apart_go(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, hipStream_t st) {
+  const auto go = [&](int rows, int tiles) {
+    if (d.q) layernorm_grad_apart_kernel<T, W, MODE, NV, true><<<rows + tiles, s.r.block, 0, st>>>(d, rows);
+    else layernorm_grad_apart_kernel<T, W, MODE, NV, false><<<rows + tiles, s.r.block, 0, st>>>(d, rows);
+    return launched();
+  };
+  if (!s.before || !s.tiles || !s.grid) return go(s.grid, s.tiles);
+  const int rc = go(0, s.tiles);
+  return rc ? rc : go(s.grid, 0);
+}
+
+template <class T, class W, int MODE, int NV, bool MULTI, bool FULL>
+int grad_go(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part, hipStream_t st) {
+  if (d.q) layernorm_grad_kernel<T, W, MODE, NV, true, MULTI, FULL><<<s.grid, s.r.block, 0, st>>>(d, part);
+  else layernorm_grad_kernel<T, W, MODE, NV, false, MULTI, FULL><<<s.grid, s.r.block, 0, st>>>(d, part);
   return launched();
+}
+
+template <class T, class W, int MODE, int NV>
+int grad_nv(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part, hipStream_t st) {
+  const bool full = d.cols % 8 == 0 && !d.y;
+  if (s.apart) return apart_go<T, W, MODE, NV>(d, s, st);
+  if (d.nsrc > 1 || d.y)
+    return full ? grad_go<T, W, MODE, NV, true, true>(d, s, part, st) : grad_go<T, W, MODE, NV, true, false>(d, s, part, st);
+  return full ? grad_go<T, W, MODE, NV, false, true>(d, s, part, st) : grad_go<T, W, MODE, NV, false, false>(d, s, part, st);
 }
 
 template <class T, class W>
 int grad_w(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part, hipStream_t st) {
-  if (s.wide) return s.nv == 4 ? grad_go<T, W, 4, 1024, 1024, false>(d, s.grid, part, st)
-                               : grad_go<T, W, 8, 1024, 1024, false>(d, s.grid, part, st);
-  if (s.tpr == 16) return grad_go<T, W, 1, 16, 256, true>(d, s.grid, part, st);
-  if (s.tpr == 64) return s.nv == 1 ? grad_go<T, W, 1, 64, 256, true>(d, s.grid, part, st)
-                                    : grad_go<T, W, 2, 64, 256, true>(d, s.grid, part, st);
-  if (s.tpr == 256) return grad_go<T, W, 1, 256, 256, true>(d, s.grid, part, st);
-  if (s.tpr == 512) return grad_go<T, W, 1, 512, 512, true>(d, s.grid, part, st);
-  return s.nv == 1 ? grad_go<T, W, 1, 1024, 1024, true>(d, s.grid, part, st)
-                   : grad_go<T, W, 2, 1024, 1024, true>(d, s.grid, part, st);
+  if (s.r.mode == 16) return grad_nv<T, W, 16, 1>(d, s, part, st);
+  if (s.r.mode == 64) return grad_nv<T, W, 64, 1>(d, s, part, st);
+  if (s.r.nv == 1) return grad_nv<T, W, 0, 1>(d, s, part, st);
+  if (s.r.nv == 2) return grad_nv<T, W, 0, 2>(d, s, part, st);
+  if (s.r.nv == 4) return grad_nv<T, W, 0, 4>(d, s, part, st);
+  // wide: the rows alone (the column sums, if any, have a launch of their own before this one)
+  if (s.r.nv == 8) return apart_go<T, W, 0, 8>(d, s, st);
+  return apart_go<T, W, 0, 16>(d, s, st);
 }
 
 template <class T>
 int grad_cols(const ext_mpi_amd_layernorm_grad &d, int slices, float *part, hipStream_t st) {
   const dim3 grid(slices, (unsigned)((d.cols + 511) / 512));
-  if (d.q && d.nsrc > 1)
-    layernorm_cols_kernel<T, true, true><<<grid, 256, 0, st>>>(d, part);
-  else if (d.q)
-    layernorm_cols_kernel<T, true, false><<<grid, 256, 0, st>>>(d, part);
-  else if (d.nsrc > 1)
-    layernorm_cols_kernel<T, false, true><<<grid, 256, 0, st>>>(d, part);
-  else
-    layernorm_cols_kernel<T, false, false><<<grid, 256, 0, st>>>(d, part);
+  if (d.q) layernorm_cols_kernel<T, true><<<grid, 256, 0, st>>>(d, part);
+  else layernorm_cols_kernel<T, false><<<grid, 256, 0, st>>>(d, part);
   return launched();
 }
 
-template <class T>
-int grad_launch(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part, hipStream_t st) {
-  int rc;
-  if (s.wide) {
-    // the column sums first: dx may overwrite what they read
-    if ((d.dweight || d.dbias) && (rc = grad_cols<T>(d, s.grid, part, st))) return rc;
-    if (!d.dx && !d.y) return 0;
-  }
-  if (d.wdtype == d.dtype || !(d.weight || d.bias)) return grad_w<T, T>(d, s, part, st);
-  return grad_w<T, float>(d, s, part, st);
-}
+// whether weights of their own type need their own kernels
+inline bool own_weights(int dtype, int wdtype, const void *w, const void *b) { return (w || b) && wdtype != dtype; }
 
 } // namespace emac_rows
 #endif

@@ -18,66 +18,175 @@ namespace emac_rows {
 typedef __bf16 bf16;
 typedef _Float16 half;
 
-template <class T>
-using v8 = T __attribute__((ext_vector_type(8)));
-template <class T>
-struct packed { // 8 elements in memory, at any element's address
-  typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-};
-typedef v8<float> f8;
-typedef unsigned short us8 __attribute__((ext_vector_type(8)));
-typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+typedef float f8 __attribute__((ext_vector_type(8)));
+typedef float f2 __attribute__((ext_vector_type(2)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
-typedef unsigned u2_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef unsigned u8x __attribute__((ext_vector_type(8)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 
-// `n` (clamped) of the 8 elements at p, zeros in the place of the others
+// 8 elements as loaded, in dwords (vectors of 16-bit types end up an element to a register where
+// they cross a branch): two elements of a 16-bit type to a dword, four bytes of a checkpoint
+template <int ESIZE>
+struct dwords;
+template <>
+struct dwords<4> { typedef u8x type; };
+template <>
+struct dwords<2> { typedef u4 type; };
+template <>
+struct dwords<1> { typedef u2 type; };
 template <class T>
-__device__ inline v8<T> load8(const T *p, long n) {
-  if (n >= 8) return *(const typename packed<T>::type *)p;
-  v8<T> r = (v8<T>)(T)0;
+using raw8 = typename dwords<sizeof(T)>::type;
+template <class V, int ALIGN>
+struct any { // V in memory at any element's address
+  typedef V type __attribute__((aligned(ALIGN)));
+};
+
+// a value that the compiler takes to be new here
+template <class V>
+__device__ inline void hold(V &v) {
 #pragma unroll
-  for (int j = 0; j < 8; j++)
-    if (j < n) r[j] = p[j];
+  for (unsigned k = 0; k < sizeof(V) / 4; k++) {
+    unsigned t = v[k];
+    asm volatile("" : "+v"(t));
+    v[k] = t;
+  }
+}
+
+// `n` (clamped) of the 8 elements at column c of a row, zeros in the place of the others (a row that
+// all lanes share is a scalar base, and c a 32-bit offset from it). Matrices pass through
+// once: nontemporal (a 4096 x 8192 norm of bf16 56 us against 65, a checkpoint of 8192 x 16384 71
+// against 90); what is read again soon is loaded and stored with `again`. A row's last elements
+// come in pieces of 1, 2 and 4 from its end, each moving up what it precedes: three branches that
+// only the row's last lane takes.
+template <class T, bool again = false>
+__device__ inline raw8<T> load8(const T *row, unsigned c, int n) {
+  constexpr int E = sizeof(T);
+  typedef raw8<T> R;
+  const char *p = (const char *)row + c * (unsigned)E;
+  if (!__builtin_constant_p(n)) asm volatile("" : "+v"(n)); // or the branches of several loads are threaded together
+  if (n >= 8) {
+    typedef typename any<R, E>::type RA;
+    if (again) return *(const RA *)p;
+    return __builtin_nontemporal_load((const RA *)p);
+  }
+  R r = (R)0u;
+  if (n <= 0) return r;
+  if constexpr (E == 4) {
+    if (n & 1) r[0] = *(const unsigned *)(p + 4 * (n & 6));
+    if (n & 2) {
+      const u2 v = *(const typename any<u2, 4>::type *)(p + 4 * (n & 4));
+      r[2] = r[0];
+      r[0] = v[0];
+      r[1] = v[1];
+    }
+    if (n & 4) {
+      const u4 v = *(const typename any<u4, 4>::type *)p;
+      r.hi = r.lo;
+      r.lo = v;
+    }
+  } else if constexpr (E == 2) {
+    if (n & 1) r[0] = *(const unsigned short *)(p + 2 * (n & 6));
+    if (n & 2) {
+      r[1] = r[0];
+      r[0] = *(const typename any<unsigned, 2>::type *)(p + 2 * (n & 4));
+    }
+    if (n & 4) {
+      r.hi = r.lo;
+      r.lo = *(const typename any<u2, 2>::type *)p;
+    }
+  } else {
+    if (n & 1) r[0] = *(const unsigned char *)(p + (n & 6));
+    if (n & 2) r[0] = r[0] << 16 | *(const typename any<unsigned short, 1>::type *)(p + (n & 4));
+    if (n & 4) {
+      r[1] = r[0];
+      r[0] = *(const typename any<unsigned, 1>::type *)p;
+    }
+  }
   return r;
 }
 
-template <class T>
-__device__ inline void store8(T *p, v8<T> v, long n) {
+template <class T, bool again = false>
+__device__ inline void store8(T *row, unsigned c, raw8<T> v, int n) {
+  constexpr int E = sizeof(T);
+  char *p = (char *)row + c * (unsigned)E;
+  if (!__builtin_constant_p(n)) asm volatile("" : "+v"(n));
   if (n >= 8) {
-    *(typename packed<T>::type *)p = v;
+    typedef typename any<raw8<T>, E>::type RA;
+    if (again) *(RA *)p = v;
+    else __builtin_nontemporal_store((RA)v, (RA *)p);
     return;
   }
-#pragma unroll
-  for (int j = 0; j < 8; j++)
-    if (j < n) p[j] = v[j];
+  if (n <= 0) return;
+  if constexpr (E == 4) {
+    if (n & 4) {
+      *(typename any<u4, 4>::type *)p = v.lo;
+      v.lo = v.hi;
+    }
+    if (n & 2) {
+      *(typename any<u2, 4>::type *)(p + 4 * (n & 4)) = v.lo.lo;
+      v[0] = v[2];
+    }
+    if (n & 1) *(unsigned *)(p + 4 * (n & 6)) = v[0];
+  } else if constexpr (E == 2) {
+    if (n & 4) {
+      *(typename any<u2, 2>::type *)p = v.lo;
+      v.lo = v.hi;
+    }
+    if (n & 2) {
+      *(typename any<unsigned, 2>::type *)(p + 2 * (n & 4)) = v[0];
+      v[0] = v[1];
+    }
+    if (n & 1) *(unsigned short *)(p + 2 * (n & 6)) = (unsigned short)v[0];
+  } else {
+    if (n & 4) {
+      *(typename any<unsigned, 1>::type *)p = v[0];
+      v[0] = v[1];
+    }
+    if (n & 2) {
+      *(typename any<unsigned short, 1>::type *)(p + (n & 4)) = (unsigned short)v[0];
+      v[0] >>= 16;
+    }
+    if (n & 1) *(unsigned char *)(p + (n & 6)) = (unsigned char)v[0];
+  }
 }
 
-__device__ inline u2 load8q(const signed char *p, long n) {
-  if (n >= 8) return *(const u2_any *)p;
-  u2 r = {0, 0};
+// between dwords and 32-bit floats; round_to rounds to nearest, ties to even
+template <class T>
+__device__ inline f8 widen(raw8<T> v) {
+  f8 r;
+  if constexpr (sizeof(T) == 4) {
+    r = __builtin_bit_cast(f8, v);
+  } else {
 #pragma unroll
-  for (int j = 0; j < 8; j++)
-    if (j < n) r[j / 4] |= (unsigned)(unsigned char)p[j] << 8 * (j % 4);
+    for (int k = 0; k < 4; k++) {
+      if constexpr (__is_same(T, bf16)) {
+        r[2 * k] = __uint_as_float(v[k] << 16);
+        r[2 * k + 1] = __uint_as_float(v[k] & 0xffff0000u);
+      } else {
+        typedef half h2 __attribute__((ext_vector_type(2)));
+        const h2 h = __builtin_bit_cast(h2, (unsigned)v[k]);
+        r[2 * k] = (float)h.x;
+        r[2 * k + 1] = (float)h.y;
+      }
+    }
+  }
   return r;
 }
-
-__device__ inline void store8q(signed char *p, u2 v, long n) {
-  if (n >= 8) {
-    *(u2_any *)p = v;
-    return;
-  }
+template <class T>
+__device__ inline raw8<T> round_to(f8 v) {
+  raw8<T> r;
+  if constexpr (sizeof(T) == 4) {
+    r = __builtin_bit_cast(u8x, v);
+  } else {
+    typedef T t2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-  for (int j = 0; j < 8; j++)
-    if (j < n) p[j] = (signed char)(v[j / 4] >> 8 * (j % 4));
-}
-
-template <class T>
-__device__ inline f8 widen(v8<T> v) {
-  return __builtin_convertvector(v, f8);
-}
-template <class T>
-__device__ inline v8<T> round_to(f8 v) {
-  return __builtin_convertvector(v, v8<T>);
+    for (int k = 0; k < 4; k++) {
+      const f2 f = {v[2 * k], v[2 * k + 1]};
+      r[k] = __builtin_bit_cast(unsigned, __builtin_convertvector(f, t2));
+    }
+  }
+  return r;
 }
 
 // ---- reductions inside a wave: DPP row rotations (16 lanes), then the four rows by readlane.
@@ -92,6 +201,12 @@ __device__ inline float row_ror(float v) {
 }
 __device__ inline float sum16(float v) {
   v += row_ror<8>(v);
+  v += row_ror<4>(v);
+  v += row_ror<2>(v);
+  v += row_ror<1>(v);
+  return v;
+}
+__device__ inline float sum8(float v) { // of lanes that hold the same eight values every eight lanes
   v += row_ror<4>(v);
   v += row_ror<2>(v);
   v += row_ror<1>(v);
@@ -114,20 +229,21 @@ __device__ inline float sum64(float v) {
 
 // ---- checkpoints: 8 bits and a float scale for each 128 columns ----
 
-// the bits of max |x| as a float's: integer order, in which an infinity and every NaN lie above
+// the bits of max |x| in its own type: integer order, in which an infinity and every NaN lie above
 // all finite values, so neither is lost in the maximum
-__device__ inline unsigned abs_bits(v8<float> x) {
-  unsigned m = 0;
-#pragma unroll
-  for (int j = 0; j < 8; j++) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
-  return m;
-}
 template <class T>
-__device__ inline unsigned abs_bits(v8<T> x) { // 16-bit types: their own bits
-  us8 u = __builtin_bit_cast(us8, x) & (us8)(unsigned short)0x7fff;
-  us2 a = __builtin_elementwise_max(u.s01, u.s23), b = __builtin_elementwise_max(u.s45, u.s67);
-  a = __builtin_elementwise_max(a, b);
-  return max((unsigned)a.x, (unsigned)a.y);
+__device__ inline unsigned abs_bits(raw8<T> x) {
+  if constexpr (sizeof(T) == 4) {
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) m = max(m, x[j] & 0x7fffffffu);
+    return m;
+  } else {
+    us2 m = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 4; k++) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2, (unsigned)x[k] & 0x7fff7fffu));
+    return max((unsigned)m.x, (unsigned)m.y);
+  }
 }
 template <class T>
 __device__ inline float of_bits(unsigned m);
@@ -153,9 +269,9 @@ struct block8 {
 // (no contraction), so the bytes are the definition's on every path. 1.5 * 2^23 added to a value
 // of magnitude <= 128 leaves its integer, ties to even, in the low byte of the sum.
 template <class T>
-__device__ inline block8 quantise(v8<T> x) {
+__device__ inline block8 quantise(raw8<T> x) {
 #pragma clang fp contract(off)
-  const float a = of_bits<T>(max16(abs_bits(x)));
+  const float a = of_bits<T>(max16(abs_bits<T>(x)));
   const bool finite = a <= 3.4028234663852886e38f;
   const float am = fmaxf(a, 0x1p-100f);
   const float inv = finite ? 127.0f / am : 0.0f;
@@ -177,13 +293,14 @@ __device__ inline block8 quantise(v8<T> x) {
   return r;
 }
 
-__device__ inline f8 restore(u2 q, float scale) {
-#pragma clang fp contract(off)
+// eight signed bytes as floats
+__device__ inline f8 bytes(u2 q) {
   f8 r;
 #pragma unroll
-  for (int j = 0; j < 8; j++) r[j] = (float)(int)(signed char)(q[j / 4] >> 8 * (j % 4)) * scale;
+  for (int j = 0; j < 8; j++) r[j] = (float)(int)(signed char)(q[j / 4] >> 8 * (j % 4));
   return r;
 }
+__device__ inline f8 restore(u2 q, float scale) { return bytes(q) * scale; }
 
 // ---- launch helper: the grid must not be empty, and a launch error is the caller's ----
 inline int launched() { return hipGetLastError() == hipSuccess ? 0 : EMAC_ERR_DEVICE; }
