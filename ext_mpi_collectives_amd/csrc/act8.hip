@@ -16,23 +16,25 @@ using namespace emac_rows;
 constexpr int kGroups = 16; // lane groups in a workgroup
 
 // ---- activations: value and slope, in 32 bits ----
-// 16-bit types take the native exp2 and reciprocal (1 ulp each); float the library's exp and IEEE
-// division, since 2 ulp of the native ones' argument rounding would show in its far tails.
+// 16-bit types take the native exp2 (of x log2 e rounded) and reciprocal, 1 ulp each. Float adds what
+// the rounded product lost, |x| ulp in the exponential's far tails, and one Newton step: the library's
+// exponential and an IEEE division make a gated SiLU of 8192 x 4096 floats 156 us instead of 90.
 template <class T>
 __device__ inline float exp_of(float x) {
-  return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f);
-}
-template <>
-__device__ inline float exp_of<float>(float x) {
-  return expf(x);
+  const float log2e = 1.44269504088896340736f;
+  if constexpr (sizeof(T) == 4) {
+    x = __builtin_amdgcn_fmed3f(x, -104.0f, 88.5f); // 0 and its reciprocal's reach: finite
+    const float y = x * log2e, lost = fmaf(x, log2e, -y) + x * 1.92596299e-8f; // log2 e - log2e
+    const float e = __builtin_amdgcn_exp2f(y);
+    return fmaf(e, lost * 0.693147181f, e);
+  }
+  return __builtin_amdgcn_exp2f(x * log2e);
 }
 template <class T>
 __device__ inline float recip(float x) {
-  return __builtin_amdgcn_rcpf(x);
-}
-template <>
-__device__ inline float recip<float>(float x) {
-  return 1.0f / x;
+  const float r = __builtin_amdgcn_rcpf(x);
+  if constexpr (sizeof(T) == 4) return fmaf(fmaf(-x, r, 1.0f), r, r);
+  return r;
 }
 
 template <class T, int KIND>
@@ -49,7 +51,7 @@ __device__ inline float act_value(float a) {
     // the normal distribution's tail, p = exp(-a^2/2) erfcx(|a|/sqrt 2) / 2, with erfcx(z) as a
     // polynomial of degree 8 in t = 1 / (1 + 0.4348731 z) without a constant term (least relative
     // error on 0 <= z <= 12, fitted here: 1.3e-7)
-    const float t = recip<T>(1.0f + 0.30750170f * fabsf(a));
+    const float t = recip<T>(1.0f + 0.30750170f * fminf(fabsf(a), 64.0f)); // beyond, e is 0
     e = exp_of<T>(-0.5f * a * a);
     p = 0.036300003528594971f;
     p = p * t - 0.14733710885047913f;
@@ -76,7 +78,7 @@ __device__ inline void act_both(float a, float &value, float &slope) {
     value = a * s;
     slope = s + value * (1.0f - s) * (1.5957691216057308f * (1.0f + 3.0f * c2));
   } else {
-    const float t = recip<T>(1.0f + 0.30750170f * fabsf(a));
+    const float t = recip<T>(1.0f + 0.30750170f * fminf(fabsf(a), 64.0f)); // beyond, e is 0
     const float e = exp_of<T>(-0.5f * a * a);
     float p = 0.036300003528594971f;
     p = p * t - 0.14733710885047913f;
@@ -94,102 +96,115 @@ __device__ inline void act_both(float a, float &value, float &slope) {
 }
 
 // where a lane's 8 elements of block `u` (0 .. U - 1) of its group lie
+template <int TAIL>
 struct place {
-  long row;
-  int blk, c; // block of the row, first column of the lane
-  int n;      // elements from there to the row's end, 0 or less if none
+  long row, from; // its row, the row loaded from (the last one again past it)
+  int blk, own, c; // block of the row, first column of the lane, the column loaded from
+  int n;           // elements from there to the row's end, 0 or less if none
+  bool in;
+  template <class T>
+  __device__ raw8<T> load(const void *p, long stride) const { // to be put() where it is used
+    const T *r = (const T *)p + from * stride;
+    if constexpr (TAIL == PIECES) return load_pieces(r + own, n);
+    else return load8(r, (unsigned)c);
+  }
+  template <class T>
+  __device__ raw8<T> put(raw8<T> v) const {
+    if constexpr (TAIL == SHIFT) return last8<T>(v, n);
+    else return TAIL == FULL && !in ? (raw8<T>)0u : v;
+  }
+  template <class T>
+  __device__ void store(void *p, long stride, raw8<T> v) const {
+    if (in) store8<T>((T *)p + row * stride, (unsigned)own, v, TAIL == FULL ? 8 : n);
+  }
 };
-template <int U>
+template <int U, int TAIL>
 struct span8 {
   long row0;
   unsigned blk0, nblk;
-  long rows, cols;
-  __device__ span8(long rows_, long cols_, unsigned nblk_) : nblk(nblk_), rows(rows_), cols(cols_) {
+  long rows;
+  int cols;
+  __device__ span8(long rows_, long cols_, unsigned nblk_) : nblk(nblk_), rows(rows_), cols((int)cols_) {
     const unsigned first = blockIdx.x * (unsigned)(U * kGroups);
     row0 = first / nblk;
     blk0 = first - (unsigned)row0 * nblk;
   }
-  __device__ place at(int u) const {
+  __device__ place<TAIL> at(int u) const {
     const unsigned x = blk0 + u * kGroups + threadIdx.x / 16;
-    place p;
+    place<TAIL> p;
     unsigned k;
     if (nblk >= (unsigned)(U * kGroups)) k = x >= nblk ? 1u : 0u;
     else k = x / nblk;
     p.row = row0 + k;
+    p.from = p.row < rows ? p.row : rows - 1;
     p.blk = (int)(x - k * nblk);
-    p.c = p.blk * EMAC_BLOCK8 + (int)(threadIdx.x % 16) * 8;
-    p.n = p.row < rows ? (int)cols - p.c : 0;
+    p.own = p.blk * EMAC_BLOCK8 + (int)(threadIdx.x % 16) * 8;
+    p.n = p.row < rows ? cols - p.own : 0;
+    p.in = p.n > 0;
+    p.c = min(p.own, cols - 8);
     return p;
   }
 };
 
-template <class T>
-__device__ inline void put8(const place &p, raw8<T> x, signed char *q, long q_stride, float *scale, unsigned nblk) {
+template <class T, int TAIL>
+__device__ inline void put8(const place<TAIL> &p, raw8<T> x, signed char *q, long q_stride, float *scale, unsigned nblk) {
   const block8 b = quantise<T>(x);
-  if (p.n > 0) {
-    store8<signed char>(q + p.row * q_stride, p.c, b.q, p.n);
-    if (threadIdx.x % 16 == 0) scale[p.row * nblk + p.blk] = b.scale;
-  }
+  p.template store<signed char>(q, q_stride, b.q);
+  if (p.in && threadIdx.x % 16 == 0) scale[p.row * nblk + p.blk] = b.scale;
 }
 
-template <class T, int KIND, bool GATE, int U>
+template <class T, int KIND, bool GATE, int U, int TAIL>
 __global__ __launch_bounds__(256) void act_kernel(const ext_mpi_amd_act d, unsigned nblk) {
-  const span8<U> s(d.rows, d.cols, nblk);
+  const span8<U, TAIL> s(d.rows, d.cols, nblk);
   raw8<T> a[U], b[GATE ? U : 1];
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const place p = s.at(u);
-    a[u] = (raw8<T>)0u;
-    if (GATE) b[GATE ? u : 0] = a[u];
-    if (p.n > 0) {
-      a[u] = load8((const T *)d.a + p.row * d.a_stride, p.c, p.n);
-      if (GATE) b[GATE ? u : 0] = load8((const T *)d.b + p.row * d.b_stride, p.c, p.n);
-    }
+    const place<TAIL> p = s.at(u);
+    a[u] = p.template load<T>(d.a, d.a_stride);
+    if (GATE) b[GATE ? u : 0] = p.template load<T>(d.b, d.b_stride);
   }
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const place p = s.at(u);
-    if (d.qa) {
-      put8<T>(p, a[u], d.qa, d.q_stride, d.sa, nblk);
-      if (GATE) put8<T>(p, b[GATE ? u : 0], d.qb, d.q_stride, d.sb, nblk);
-    }
+    const place<TAIL> p = s.at(u);
+    const raw8<T> av = p.template put<T>(a[u]), bv = p.template put<T>(b[GATE ? u : 0]);
     if constexpr (KIND != EMAC_SAVE8) {
-      if (d.h && p.n > 0) {
-        const f8 f = widen<T>(a[u]);
+      if (d.h) {
+        const f8 f = widen<T>(av);
         f8 v;
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = act_value<T, KIND>(f[j]);
-        if (GATE) v *= widen<T>(b[GATE ? u : 0]);
-        store8<T>((T *)d.h + p.row * d.h_stride, p.c, round_to<T>(v), p.n);
+        if (GATE) v *= widen<T>(bv);
+        p.template store<T>(d.h, d.h_stride, round_to<T>(v));
       }
+    }
+    if (d.qa) {
+      put8<T>(p, av, d.qa, d.q_stride, d.sa, nblk);
+      if (GATE) put8<T>(p, bv, d.qb, d.q_stride, d.sb, nblk);
     }
   }
 }
 
-template <class T, int KIND, bool GATE, int U>
+template <class T, int KIND, bool GATE, int U, int TAIL>
 __global__ __launch_bounds__(256) void act_grad_kernel(const ext_mpi_amd_act_grad d, unsigned nblk) {
-  const span8<U> s(d.rows, d.cols, nblk);
+  const span8<U, TAIL> s(d.rows, d.cols, nblk);
   raw8<T> g[U];
   u2 qa[U], qb[GATE ? U : 1];
   float sa[U], sb[GATE ? U : 1];
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const place p = s.at(u);
-    if (p.n > 0) {
-      g[u] = load8((const T *)d.dh + p.row * d.dh_stride, p.c, p.n);
-      qa[u] = load8<signed char>(d.qa + p.row * d.q_stride, p.c, p.n);
-      sa[u] = d.sa[p.row * nblk + p.blk];
-      if (GATE) {
-        qb[GATE ? u : 0] = load8<signed char>(d.qb + p.row * d.q_stride, p.c, p.n);
-        sb[GATE ? u : 0] = d.sb[p.row * nblk + p.blk];
-      }
+    const place<TAIL> p = s.at(u);
+    g[u] = p.template load<T>(d.dh, d.dh_stride);
+    qa[u] = p.template load<signed char>(d.qa, d.q_stride);
+    sa[u] = d.sa[p.from * nblk + p.blk];
+    if (GATE) {
+      qb[GATE ? u : 0] = p.template load<signed char>(d.qb, d.q_stride);
+      sb[GATE ? u : 0] = d.sb[p.from * nblk + p.blk];
     }
   }
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const place p = s.at(u);
-    if (p.n <= 0) continue;
-    const f8 a = restore(qa[u], sa[u]), dh = widen<T>(g[u]);
+    const place<TAIL> p = s.at(u);
+    const f8 a = restore(p.template put<signed char>(qa[u]), sa[u]), dh = widen<T>(p.template put<T>(g[u]));
     f8 value, slope;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -200,35 +215,33 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const ext_mpi_amd_act_gra
     }
     slope *= dh;
     if (GATE) {
-      const f8 b = restore(qb[GATE ? u : 0], sb[GATE ? u : 0]);
-      store8<T>((T *)d.da + p.row * d.da_stride, p.c, round_to<T>(slope * b), p.n);
-      store8<T>((T *)d.db + p.row * d.db_stride, p.c, round_to<T>(dh * value), p.n);
+      const f8 b = restore(p.template put<signed char>(qb[GATE ? u : 0]), sb[GATE ? u : 0]);
+      p.template store<T>(d.da, d.da_stride, round_to<T>(slope * b));
+      p.template store<T>(d.db, d.db_stride, round_to<T>(dh * value));
       value *= b;
     } else {
-      store8<T>((T *)d.da + p.row * d.da_stride, p.c, round_to<T>(slope), p.n);
+      p.template store<T>(d.da, d.da_stride, round_to<T>(slope));
     }
-    if (d.h) store8<T>((T *)d.h + p.row * d.h_stride, p.c, round_to<T>(value), p.n);
+    if (d.h) p.template store<T>(d.h, d.h_stride, round_to<T>(value));
   }
 }
 
-template <class T, int U>
+template <class T, int U, int TAIL>
 __global__ __launch_bounds__(256) void restore8_kernel(long rows, long cols, const signed char *q, long q_stride,
                                                        const float *scale, T *x, long x_stride, unsigned nblk) {
-  const span8<U> s(rows, cols, nblk);
+  const span8<U, TAIL> s(rows, cols, nblk);
   u2 w[U];
   float sc[U];
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const place p = s.at(u);
-    if (p.n > 0) {
-      w[u] = load8<signed char>(q + p.row * q_stride, p.c, p.n);
-      sc[u] = scale[p.row * nblk + p.blk];
-    }
+    const place<TAIL> p = s.at(u);
+    w[u] = p.template load<signed char>(q, q_stride);
+    sc[u] = scale[p.from * nblk + p.blk];
   }
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const place p = s.at(u);
-    if (p.n > 0) store8<T>(x + p.row * x_stride, p.c, round_to<T>(restore(w[u], sc[u])), p.n);
+    const place<TAIL> p = s.at(u);
+    p.template store<T>(x, x_stride, round_to<T>(restore(p.template put<signed char>(w[u]), sc[u])));
   }
 }
 
@@ -236,23 +249,36 @@ __global__ __launch_bounds__(256) void restore8_kernel(long rows, long cols, con
 
 struct grid8 {
   unsigned nblk, grid;
-  int u;
+  int u, tail;
 };
 // blocks, workgroups and blocks per lane group (engine_rows.c holds rows * blocks under 2^31): 4
 // blocks' loads in flight where that leaves 8 workgroups to a CU, else as many workgroups as can be
-grid8 grid_of(long rows, long cols) {
+grid8 grid_of(long rows, long cols, bool in_place) {
   grid8 g;
   g.nblk = (unsigned)((cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8);
-  g.u = rows * g.nblk >= 4L * kGroups * 2048 ? 4 : 1;
+  g.tail = tail_of(cols);
+  if (g.tail == SHIFT && in_place) g.tail = PIECES;
+  g.u = g.tail != PIECES && rows * g.nblk >= 4L * kGroups * 2048 ? 4 : 1;
   g.grid = (unsigned)((rows * g.nblk + g.u * kGroups - 1) / (g.u * kGroups));
   return g;
 }
 
+template <int V>
+struct num {
+  static constexpr int v = V;
+};
+// calls go with the kernel's U and TAIL
+template <class F>
+void shaped(const grid8 &g, F go) {
+  if (g.tail == PIECES) go(num<1>(), num<PIECES>());
+  else if (g.tail == FULL) g.u == 4 ? go(num<4>(), num<FULL>()) : go(num<1>(), num<FULL>());
+  else g.u == 4 ? go(num<4>(), num<SHIFT>()) : go(num<1>(), num<SHIFT>());
+}
+
 template <class T, int KIND, bool GATE>
 int act_go(const ext_mpi_amd_act &d, hipStream_t st) {
-  const grid8 g = grid_of(d.rows, d.cols);
-  if (g.u == 4) act_kernel<T, KIND, GATE, 4><<<g.grid, 256, 0, st>>>(d, g.nblk);
-  else act_kernel<T, KIND, GATE, 1><<<g.grid, 256, 0, st>>>(d, g.nblk);
+  const grid8 g = grid_of(d.rows, d.cols, d.h && (d.h == d.a || d.h == d.b));
+  shaped(g, [&](auto u, auto tail) { act_kernel<T, KIND, GATE, u.v, tail.v><<<g.grid, 256, 0, st>>>(d, g.nblk); });
   return launched();
 }
 
@@ -274,9 +300,8 @@ int act_t(const ext_mpi_amd_act &d, hipStream_t st) {
 
 template <class T, int KIND, bool GATE>
 int act_grad_go(const ext_mpi_amd_act_grad &d, hipStream_t st) {
-  const grid8 g = grid_of(d.rows, d.cols);
-  if (g.u == 4) act_grad_kernel<T, KIND, GATE, 4><<<g.grid, 256, 0, st>>>(d, g.nblk);
-  else act_grad_kernel<T, KIND, GATE, 1><<<g.grid, 256, 0, st>>>(d, g.nblk);
+  const grid8 g = grid_of(d.rows, d.cols, d.da == d.dh || d.db == d.dh || d.h == d.dh);
+  shaped(g, [&](auto u, auto tail) { act_grad_kernel<T, KIND, GATE, u.v, tail.v><<<g.grid, 256, 0, st>>>(d, g.nblk); });
   return launched();
 }
 
@@ -298,9 +323,10 @@ int act_grad_t(const ext_mpi_amd_act_grad &d, hipStream_t st) {
 template <class T>
 int restore_t(long rows, long cols, const signed char *q, long q_stride, const float *scale, void *x, long x_stride,
               hipStream_t st) {
-  const grid8 g = grid_of(rows, cols);
-  if (g.u == 4) restore8_kernel<T, 4><<<g.grid, 256, 0, st>>>(rows, cols, q, q_stride, scale, (T *)x, x_stride, g.nblk);
-  else restore8_kernel<T, 1><<<g.grid, 256, 0, st>>>(rows, cols, q, q_stride, scale, (T *)x, x_stride, g.nblk);
+  const grid8 g = grid_of(rows, cols, false);
+  shaped(g, [&](auto u, auto tail) {
+    restore8_kernel<T, u.v, tail.v><<<g.grid, 256, 0, st>>>(rows, cols, q, q_stride, scale, (T *)x, x_stride, g.nblk);
+  });
   return launched();
 }
 

@@ -34,25 +34,30 @@ struct lanes {
   }
 };
 
-// A lane's vector i of a row. FULL (cols a multiple of 8): a vector lies inside the row or past it,
-// and a lane past it loads the row's last vector again, which is kept out of every sum and store --
-// no load has a branch. Else the last vector holds `n` elements and zeros.
-template <bool FULL>
+// A lane's vector i of a row. A lane past the row's end loads the row's last vector again: with
+// SHIFT that is zeros once moved into place, with FULL it is kept out of every sum and store.
+template <int TAIL>
 struct slot {
-  int c, n; // column, elements (0 or less: none)
+  int own, c, n; // first column, the column loaded from, elements (0 or less: none)
   __device__ slot(int i, int per, int l, int cols, bool live) {
-    const int at = (l + i * per) * 8;
-    n = live ? cols - at : 0;
-    c = FULL && at >= cols ? cols - 8 : at;
+    own = (l + i * per) * 8;
+    n = live ? cols - own : 0;
+    c = min(own, cols - 8);
   }
   __device__ bool in() const { return n > 0; }
   template <class T, bool again = false>
-  __device__ raw8<T> load(const void *row) const {
-    return load8<T, again>((const T *)row, (unsigned)c, FULL ? 8 : n);
+  __device__ raw8<T> load(const void *row) const { // to be put() where it is used
+    if constexpr (TAIL == PIECES) return load_pieces((const T *)row + own, n);
+    else return load8<T, again>((const T *)row, (unsigned)c);
+  }
+  template <class T>
+  __device__ raw8<T> put(raw8<T> v) const {
+    if constexpr (TAIL == SHIFT) return last8<T>(v, n);
+    else return v;
   }
   template <class T>
   __device__ void store(void *row, raw8<T> v) const {
-    if (in()) store8<T>((T *)row, (unsigned)c, v, FULL ? 8 : n);
+    if (in()) store8<T>((T *)row, (unsigned)own, v, TAIL == FULL ? 8 : n);
   }
 };
 template <class T>
@@ -93,8 +98,8 @@ struct row_sum {
 };
 
 // ((leaf 0 + leaf 1) + ...) of 8 elements in 32 bits, the loads of a batch in flight together
-template <class T, bool FULL>
-__device__ inline f8 fold8(const void *const *src, int nsrc, long row, long stride, const slot<FULL> &at) {
+template <class T, int TAIL>
+__device__ inline f8 fold8(const void *const *src, int nsrc, long row, long stride, const slot<TAIL> &at) {
   constexpr int B = sizeof(T) == 2 ? 8 : 4;
   f8 s = {};
   for (int t0 = 0; t0 < nsrc; t0 += B) {
@@ -104,7 +109,7 @@ __device__ inline f8 fold8(const void *const *src, int nsrc, long row, long stri
       if (t0 + k < nsrc) raw[k] = at.template load<T>(row_of<T>(src[t0 + k], row, stride));
 #pragma unroll
     for (int k = 0; k < B; k++)
-      if (t0 + k < nsrc) s = t0 + k ? s + widen<T>(raw[k]) : widen<T>(raw[k]);
+      if (t0 + k < nsrc) s = t0 + k ? s + widen<T>(at.template put<T>(raw[k])) : widen<T>(at.template put<T>(raw[k]));
   }
   return s;
 }
@@ -113,7 +118,7 @@ __device__ inline f8 fold8(const void *const *src, int nsrc, long row, long stri
 // to two vectors to a lane, else (AHEAD) as loaded. A load of them among the next row's would be worse
 // than its own latency: loads return in order, so waiting for it is waiting for the next row. Only the
 // forms that do not load ahead load them at their use. ZERO: zeros past the row's end.
-template <class W, int NV, bool FULL, bool ZERO, bool AHEAD>
+template <class W, int NV, int TAIL, bool ZERO, bool AHEAD>
 struct weights {
   static constexpr bool kFloats = NV <= 2, kRaw = !kFloats && AHEAD;
   f8 v[kFloats ? NV : 1];
@@ -123,17 +128,17 @@ struct weights {
   __device__ weights(const void *p_, float none_, int per, int l, int cols) : p((const W *)p_), none(none_) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const slot<FULL> at(i, per, l, cols, true);
+      const slot<TAIL> at(i, per, l, cols, true);
       if (kFloats) v[kFloats ? i : 0] = floats(p ? at.template load<W, true>(p) : (raw8<W>)0u, at);
       if (kRaw && p) r[kRaw ? i : 0] = at.template load<W, true>(p);
     }
   }
-  __device__ f8 floats(raw8<W> w, const slot<FULL> &at) const {
-    f8 f = p ? widen<W>(w) : (f8)none;
+  __device__ f8 floats(raw8<W> w, const slot<TAIL> &at) const {
+    f8 f = p ? widen<W>(at.template put<W>(w)) : (f8)none;
     if (ZERO && !at.in()) f = (f8)0.0f;
     return f;
   }
-  __device__ f8 at(int i, const slot<FULL> &s) const {
+  __device__ f8 at(int i, const slot<TAIL> &s) const {
     if (kFloats) return v[kFloats ? i : 0];
     raw8<W> w = (raw8<W>)0u;
     if (kRaw) {
@@ -146,7 +151,7 @@ struct weights {
   }
 };
 
-template <class T, class W, int MODE, int NV, bool MULTI, bool FULL>
+template <class T, class W, int MODE, int NV, bool MULTI, int TAIL>
 __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void layernorm_kernel(const ext_mpi_amd_layernorm d) {
   constexpr bool AHEAD = !MULTI && NV * sizeof(T) <= 8; // the next row's loads are issued before this row's sums
   const lanes<MODE> ln;
@@ -155,13 +160,13 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
   const float inv = 1.0f / (float)cols;
   __shared__ float red[2][8][1];
   row_sum<MODE, 1> sum_row(red);
-  const weights<W, NV, FULL, false, AHEAD> w(d.weight, 1.0f, per, l, cols), b(d.bias, 0.0f, per, l, cols);
+  const weights<W, NV, TAIL, false, AHEAD> w(d.weight, 1.0f, per, l, cols), b(d.bias, 0.0f, per, l, cols);
   const long step = (long)gridDim.x * ln.kRows;
   raw8<T> nx[MULTI ? 1 : NV], nr[NV];
   const auto load = [&](long row) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const slot<FULL> at(i, per, l, cols, true);
+      const slot<TAIL> at(i, per, l, cols, true);
       if (!MULTI) nx[MULTI ? 0 : i] = at.template load<T>(row_of<T>(d.src[0], row, d.src_stride));
       if (d.residual) nr[i] = at.template load<T>(row_of<T>(d.residual, row, d.residual_stride));
     }
@@ -178,17 +183,17 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
     if (!AHEAD) load(within(row));
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const slot<FULL> at(i, per, l, cols, true);
+      const slot<TAIL> at(i, per, l, cols, true);
       if (MULTI || d.residual) {
         f8 f;
         if (MULTI) f = fold8<T>(d.src, d.nsrc, within(row), d.src_stride, at);
-        else f = widen<T>(nx[MULTI ? 0 : i]);
-        if (d.residual) f += widen<T>(nr[i]);
+        else f = widen<T>(at.template put<T>(nx[MULTI ? 0 : i]));
+        if (d.residual) f += widen<T>(at.template put<T>(nr[i]));
         x[i] = round_to<T>(f);
       } else {
-        x[i] = nx[MULTI ? 0 : i];
+        x[i] = at.template put<T>(nx[MULTI ? 0 : i]);
       }
-      if (FULL && !at.in()) x[i] = (raw8<T>)0u;
+      if (TAIL == FULL && !at.in()) x[i] = (raw8<T>)0u;
     }
     if (AHEAD) load(within(row + step));
 #pragma unroll
@@ -203,11 +208,11 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
       s[0] = 0.0f;
 #pragma unroll
       for (int i = 0; i < NV; i++) {
-        const slot<FULL> at(i, per, l, cols, true);
+        const slot<TAIL> at(i, per, l, cols, true);
         const f8 f = widen<T>(x[i]) - mean;
         float t = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) t += FULL || j < at.n ? f[j] * f[j] : 0.0f;
+        for (int j = 0; j < 8; j++) t += TAIL == FULL || j < at.n ? f[j] * f[j] : 0.0f;
         s[0] += at.in() ? t : 0.0f;
       }
       sum_row(s);
@@ -218,20 +223,22 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
       }
 #pragma unroll
       for (int i = 0; i < NV; i++) {
-        const slot<FULL> at(i, per, l, cols, live);
+        const slot<TAIL> at(i, per, l, cols, live);
         if (!d.y) continue;
         const f8 f = (widen<T>(x[i]) - mean) * rstd * w.at(i, at) + b.at(i, at);
         at.template store<T>((T *)d.y + row * d.y_stride, round_to<T>(f));
       }
+    } else if (MODE == 0 && TAIL == SHIFT) {
+      __syncthreads(); // sum may replace the residual: the row's last lane has read what the one before it owns
     }
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const slot<FULL> at(i, per, l, cols, live);
+      const slot<TAIL> at(i, per, l, cols, live);
       if (d.sum) at.template store<T>((T *)d.sum + row * d.sum_stride, x[i]);
       if (d.q) { // every lane of a block takes part; lanes past the row hold zeros
         const block8 k = quantise<T>(x[i]);
         at.template store<signed char>(d.q + row * d.q_stride, k.q);
-        if (at.in() && at.c % EMAC_BLOCK8 == 0) d.scale[row * nblk + at.c / EMAC_BLOCK8] = k.scale;
+        if (at.in() && at.own % EMAC_BLOCK8 == 0) d.scale[row * nblk + at.own / EMAC_BLOCK8] = k.scale;
       }
     }
   }
@@ -271,38 +278,38 @@ __device__ inline void put_cols(const ext_mpi_amd_layernorm_grad &d, float *part
 }
 
 // x of a row, or its checkpoint, as loaded
-template <class T, bool Q8, bool FULL>
+template <class T, bool Q8, int TAIL>
 struct row8 {
   raw8<T> x;
   u2 q;
   float scale;
-  __device__ void load(const ext_mpi_amd_layernorm_grad &d, long row, const slot<FULL> &at, int nblk) {
+  __device__ void load(const ext_mpi_amd_layernorm_grad &d, long row, const slot<TAIL> &at, int nblk) {
     if (Q8) {
       q = at.template load<signed char>(d.q + row * d.q_stride);
-      scale = d.scale[row * nblk + min(at.c / EMAC_BLOCK8, nblk - 1)];
+      scale = d.scale[row * nblk + min(at.own / EMAC_BLOCK8, nblk - 1)];
     } else {
       x = at.template load<T>(row_of<T>(d.x, row, d.x_stride));
     }
   }
   // (x - mean) * rstd, as x * rstd - mean * rstd: two roundings of the products' size
-  __device__ f8 normed(float rstd, float shift) const {
+  __device__ f8 normed(float rstd, float shift, const slot<TAIL> &at) const {
     if constexpr (Q8) {
       const float s = scale * rstd;
-      return bytes(q) * s + shift;
+      return bytes(at.template put<signed char>(q)) * s + shift;
     } else {
-      return widen<T>(x) * rstd + shift;
+      return widen<T>(at.template put<T>(x)) * rstd + shift;
     }
   }
 };
 
 // The rows of workgroup `block` of `blocks`: dx, y, and with ACC the two column sums.
-template <class T, class W, int MODE, int NV, bool Q8, bool MULTI, bool FULL, bool ACC>
+template <class T, class W, int MODE, int NV, bool Q8, bool MULTI, int TAIL, bool ACC>
 __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block, int blocks, float *part) {
   // one leaf: the next row's loads are issued before this row's sums, as far as registers go
   constexpr bool AHEAD = !MULTI && NV <= 2;
   // y has kernels of its own (the ones for any number of leaves and any width): a load of the bias
   // among the next row's, even where no y is asked for, makes every row wait for the next
-  constexpr bool Y = MULTI && !FULL;
+  constexpr bool Y = MULTI && TAIL != FULL;
   const lanes<MODE> ln;
   const int l = ln.l, per = ln.per, cols = (int)d.cols;
   const int nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
@@ -310,19 +317,19 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
   __shared__ float red[2][8][2];
   row_sum<MODE, 2> sum_row(red);
   // zeros past the row's end: what a lane there loads enters no sum of the row
-  const weights<W, NV, FULL, true, AHEAD> w(d.weight, 1.0f, per, l, cols);
+  const weights<W, NV, TAIL, true, AHEAD> w(d.weight, 1.0f, per, l, cols);
   const long step = (long)blocks * ln.kRows;
   const bool more = d.dsum && d.dx;
   f8 aw[ACC ? NV : 1] = {}, ab[ACC ? NV : 1] = {};
   raw8<T> ng[MULTI ? 1 : NV], nd[NV];
-  row8<T, Q8, FULL> nx[NV];
+  row8<T, Q8, TAIL> nx[NV];
   float nmean, nrstd;
   const auto load = [&](long row) {
     nmean = d.mean[row];
     nrstd = d.rstd[row];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const slot<FULL> at(i, per, l, cols, true);
+      const slot<TAIL> at(i, per, l, cols, true);
       if (!MULTI) ng[MULTI ? 0 : i] = at.template load<T>(row_of<T>(d.dy[0], row, d.dy_stride));
       nx[i].load(d, row, at, nblk);
       if (more) nd[i] = at.template load<T>(row_of<T>(d.dsum, row, d.dsum_stride));
@@ -341,17 +348,17 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const slot<FULL> at(i, per, l, cols, true);
+      const slot<TAIL> at(i, per, l, cols, true);
       if (MULTI) g[i] = fold8<T>(d.dy, d.nsrc, within(row), d.dy_stride, at);
-      else g[i] = widen<T>(ng[MULTI ? 0 : i]);
+      else g[i] = widen<T>(at.template put<T>(ng[MULTI ? 0 : i]));
       if (MODE != 0 && !live) g[i] = (f8)0.0f; // a row past the last
-      xh[i] = nx[i].normed(rstd, shift);
+      xh[i] = nx[i].normed(rstd, shift, at);
       dsum[i] = nd[i];
     }
     if (AHEAD) load(within(row + step));
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const slot<FULL> at(i, per, l, cols, live);
+      const slot<TAIL> at(i, per, l, cols, live);
       const f8 ww = w.at(i, at);
       if (ACC) {
         aw[ACC ? i : 0] += g[i] * xh[i];
@@ -359,7 +366,7 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
       }
       if (Y && d.y) {
         f8 y = xh[i] * ww;
-        if (d.bias) y += widen<W>(at.template load<W, true>(d.bias));
+        if (d.bias) y += widen<W>(at.template put<W>(at.template load<W, true>(d.bias)));
         at.template store<T>((T *)d.y + row * d.y_stride, round_to<T>(y));
       }
       g[i] *= ww;
@@ -374,10 +381,10 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
     const float c1 = -s[0] * inv * rstd, c2 = -s[1] * inv * rstd;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const slot<FULL> at(i, per, l, cols, live);
+      const slot<TAIL> at(i, per, l, cols, live);
       f8 dx = xh[i] * c2 + c1;
       dx += g[i] * rstd;
-      if (more) dx += widen<T>(dsum[i]);
+      if (more) dx += widen<T>(at.template put<T>(dsum[i]));
       at.template store<T>((T *)d.dx + row * d.dx_stride, round_to<T>(dx));
     }
   }
@@ -410,31 +417,31 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
   }
 }
 
-template <class T, class W, int MODE, int NV, bool Q8, bool MULTI, bool FULL>
+template <class T, class W, int MODE, int NV, bool Q8, bool MULTI, int TAIL>
 __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void layernorm_grad_kernel(
     const ext_mpi_amd_layernorm_grad d, float *part) {
-  grad_rows<T, W, MODE, NV, Q8, MULTI, FULL, true>(d, blockIdx.x, gridDim.x, part);
+  grad_rows<T, W, MODE, NV, Q8, MULTI, TAIL, true>(d, blockIdx.x, gridDim.x, part);
 }
 
 // The column sums alone: a workgroup takes 8 * LANES columns of every slices'th group of rows, as
 // many rows at a time as it has lanes for. `part` as in put_cols.
-template <class T, int LANES, bool Q8, bool MULTI, bool FULL>
+template <class T, int LANES, bool Q8, bool MULTI, int TAIL>
 __device__ inline void cols_tile(const ext_mpi_amd_layernorm_grad &d, int tile, int slice, int slices, float *part) {
   constexpr int C = 8 * LANES;
   __shared__ float comb[2][512 / LANES][C];
   const int l = threadIdx.x % LANES, k0 = threadIdx.x / LANES, R = blockDim.x / LANES;
   const int cols = (int)d.cols, nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
-  const slot<FULL> at(0, 0, tile * LANES + l, cols, true);
+  const slot<TAIL> at(0, 0, tile * LANES + l, cols, true);
   f8 aw = {}, ab = {};
 #pragma unroll 4
   for (long row = (long)slice * R + k0; row < d.rows; row += (long)slices * R) {
-    row8<T, Q8, FULL> x;
+    row8<T, Q8, TAIL> x;
     x.load(d, row, at, nblk);
     const float rstd = d.rstd[row], mean = d.mean[row];
     f8 g;
     if (MULTI) g = fold8<T>(d.dy, d.nsrc, row, d.dy_stride, at);
-    else g = widen<T>(at.template load<T>(row_of<T>(d.dy[0], row, d.dy_stride)));
-    aw += g * x.normed(rstd, -mean * rstd);
+    else g = widen<T>(at.template put<T>(at.template load<T>(row_of<T>(d.dy[0], row, d.dy_stride))));
+    aw += g * x.normed(rstd, -mean * rstd, at);
     ab += g;
   }
 #pragma unroll
@@ -458,17 +465,17 @@ __device__ inline void cols_tile(const ext_mpi_amd_layernorm_grad &d, int tile, 
 // grid: slices (x), column tiles (y).
 template <class T, bool Q8>
 __global__ __launch_bounds__(256) void layernorm_cols_kernel(const ext_mpi_amd_layernorm_grad d, float *part) {
-  cols_tile<T, 64, Q8, true, false>(d, blockIdx.y, blockIdx.x, gridDim.x, part);
+  cols_tile<T, 64, Q8, true, SHIFT>(d, blockIdx.y, blockIdx.x, gridDim.x, part);
 }
 
 // Rows without column sums, and in the workgroups behind theirs (from `blocks` on) the column sums of
 // 64 columns each over all rows: the rows are read twice, but nothing waits for anything.
-template <class T, class W, int MODE, int NV, bool Q8>
+template <class T, class W, int MODE, int NV, bool Q8, int TAIL>
 __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void layernorm_grad_apart_kernel(
     const ext_mpi_amd_layernorm_grad d, int blocks) {
-  if ((int)blockIdx.x < blocks) grad_rows<T, W, MODE, NV, Q8, true, false, false>(d, blockIdx.x, blocks, nullptr);
-  else if (d.nsrc == 1 && d.cols % 8 == 0) cols_tile<T, 8, Q8, false, true>(d, blockIdx.x - blocks, 0, 1, nullptr);
-  else cols_tile<T, 8, Q8, true, false>(d, blockIdx.x - blocks, 0, 1, nullptr);
+  if ((int)blockIdx.x < blocks) grad_rows<T, W, MODE, NV, Q8, true, TAIL, false>(d, blockIdx.x, blocks, nullptr);
+  else if (TAIL == SHIFT && d.nsrc == 1 && d.cols % 8 == 0) cols_tile<T, 8, Q8, false, FULL>(d, blockIdx.x - blocks, 0, 1, nullptr);
+  else cols_tile<T, 8, Q8, true, TAIL>(d, blockIdx.x - blocks, 0, 1, nullptr);
 }
 
 // ---- launches ----
@@ -488,34 +495,35 @@ inline row_shape row_shape_of(long cols) {
   return s;
 }
 
-template <class T, class W, int MODE, int NV, bool MULTI, bool FULL>
+template <class T, class W, int MODE, int NV, bool MULTI, int TAIL>
 int norm_go(const ext_mpi_amd_layernorm &d, const row_shape &s, hipStream_t st) {
   constexpr int rows = lanes<MODE>::kRows;
   const long want = (d.rows + rows - 1) / rows;
   const long most = (long)EMAC_NORM_CUS * ((512 + s.block - 1) / s.block); // 8 waves to a CU, or a few more
   const int grid = (int)(want < most ? want : most);
-  layernorm_kernel<T, W, MODE, NV, MULTI, FULL><<<grid, s.block, 0, st>>>(d);
+  layernorm_kernel<T, W, MODE, NV, MULTI, TAIL><<<grid, s.block, 0, st>>>(d);
   return launched();
 }
 
 template <class T, class W, int MODE, int NV>
 int norm_nv(const ext_mpi_amd_layernorm &d, const row_shape &s, hipStream_t st) {
   const bool full = d.cols % 8 == 0;
-  if (d.nsrc > 1) return full ? norm_go<T, W, MODE, NV, true, true>(d, s, st) : norm_go<T, W, MODE, NV, true, false>(d, s, st);
-  return full ? norm_go<T, W, MODE, NV, false, true>(d, s, st) : norm_go<T, W, MODE, NV, false, false>(d, s, st);
+  if (d.nsrc > 1) return full ? norm_go<T, W, MODE, NV, true, FULL>(d, s, st) : norm_go<T, W, MODE, NV, true, SHIFT>(d, s, st);
+  return full ? norm_go<T, W, MODE, NV, false, FULL>(d, s, st) : norm_go<T, W, MODE, NV, false, SHIFT>(d, s, st);
 }
 
 template <class T, class W>
 int norm_w(const ext_mpi_amd_layernorm &d, hipStream_t st) {
   const row_shape s = row_shape_of(d.cols);
+  if (tail_of(d.cols) == PIECES) return norm_go<T, W, 16, 1, true, PIECES>(d, s, st);
   if (s.mode == 16) return norm_nv<T, W, 16, 1>(d, s, st);
   if (s.mode == 64) return norm_nv<T, W, 64, 1>(d, s, st);
   if (s.nv == 1) return norm_nv<T, W, 0, 1>(d, s, st);
   if (s.nv == 2) return norm_nv<T, W, 0, 2>(d, s, st);
   if (s.nv == 4) return norm_nv<T, W, 0, 4>(d, s, st);
   // wider: the forms that take any number of leaves and any width
-  if (s.nv == 8) return norm_go<T, W, 0, 8, true, false>(d, s, st);
-  return norm_go<T, W, 0, 16, true, false>(d, s, st);
+  if (s.nv == 8) return norm_go<T, W, 0, 8, true, SHIFT>(d, s, st);
+  return norm_go<T, W, 0, 16, true, SHIFT>(d, s, st);
 }
 
 // the gradient's launch: `grid` workgroups take the rows, and each leaves a partial row of column
@@ -549,11 +557,11 @@ inline grad_shape grad_shape_of(const ext_mpi_amd_layernorm_grad &d) {
   return s;
 }
 
-template <class T, class W, int MODE, int NV>
+template <class T, class W, int MODE, int NV, int TAIL>
 int apart_go(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, hipStream_t st) {
   const auto go = [&](int rows, int tiles) {
-    if (d.q) layernorm_grad_apart_kernel<T, W, MODE, NV, true><<<rows + tiles, s.r.block, 0, st>>>(d, rows);
-    else layernorm_grad_apart_kernel<T, W, MODE, NV, false><<<rows + tiles, s.r.block, 0, st>>>(d, rows);
+    if (d.q) layernorm_grad_apart_kernel<T, W, MODE, NV, true, TAIL><<<rows + tiles, s.r.block, 0, st>>>(d, rows);
+    else layernorm_grad_apart_kernel<T, W, MODE, NV, false, TAIL><<<rows + tiles, s.r.block, 0, st>>>(d, rows);
     return launched();
   };
   if (!s.before || !s.tiles || !s.grid) return go(s.grid, s.tiles);
@@ -561,32 +569,34 @@ int apart_go(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, hipStream
   return rc ? rc : go(s.grid, 0);
 }
 
-template <class T, class W, int MODE, int NV, bool MULTI, bool FULL>
+template <class T, class W, int MODE, int NV, bool MULTI, int TAIL>
 int grad_go(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part, hipStream_t st) {
-  if (d.q) layernorm_grad_kernel<T, W, MODE, NV, true, MULTI, FULL><<<s.grid, s.r.block, 0, st>>>(d, part);
-  else layernorm_grad_kernel<T, W, MODE, NV, false, MULTI, FULL><<<s.grid, s.r.block, 0, st>>>(d, part);
+  if (d.q) layernorm_grad_kernel<T, W, MODE, NV, true, MULTI, TAIL><<<s.grid, s.r.block, 0, st>>>(d, part);
+  else layernorm_grad_kernel<T, W, MODE, NV, false, MULTI, TAIL><<<s.grid, s.r.block, 0, st>>>(d, part);
   return launched();
 }
 
 template <class T, class W, int MODE, int NV>
 int grad_nv(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part, hipStream_t st) {
   const bool full = d.cols % 8 == 0 && !d.y;
-  if (s.apart) return apart_go<T, W, MODE, NV>(d, s, st);
+  if (s.apart) return apart_go<T, W, MODE, NV, SHIFT>(d, s, st);
   if (d.nsrc > 1 || d.y)
-    return full ? grad_go<T, W, MODE, NV, true, true>(d, s, part, st) : grad_go<T, W, MODE, NV, true, false>(d, s, part, st);
-  return full ? grad_go<T, W, MODE, NV, false, true>(d, s, part, st) : grad_go<T, W, MODE, NV, false, false>(d, s, part, st);
+    return full ? grad_go<T, W, MODE, NV, true, FULL>(d, s, part, st) : grad_go<T, W, MODE, NV, true, SHIFT>(d, s, part, st);
+  return full ? grad_go<T, W, MODE, NV, false, FULL>(d, s, part, st) : grad_go<T, W, MODE, NV, false, SHIFT>(d, s, part, st);
 }
 
 template <class T, class W>
 int grad_w(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part, hipStream_t st) {
+  if (tail_of(d.cols) == PIECES)
+    return s.apart ? apart_go<T, W, 16, 1, PIECES>(d, s, st) : grad_go<T, W, 16, 1, true, PIECES>(d, s, part, st);
   if (s.r.mode == 16) return grad_nv<T, W, 16, 1>(d, s, part, st);
   if (s.r.mode == 64) return grad_nv<T, W, 64, 1>(d, s, part, st);
   if (s.r.nv == 1) return grad_nv<T, W, 0, 1>(d, s, part, st);
   if (s.r.nv == 2) return grad_nv<T, W, 0, 2>(d, s, part, st);
   if (s.r.nv == 4) return grad_nv<T, W, 0, 4>(d, s, part, st);
   // wide: the rows alone (the column sums, if any, have a launch of their own before this one)
-  if (s.r.nv == 8) return apart_go<T, W, 0, 8>(d, s, st);
-  return apart_go<T, W, 0, 16>(d, s, st);
+  if (s.r.nv == 8) return apart_go<T, W, 0, 8, SHIFT>(d, s, st);
+  return apart_go<T, W, 0, 16, SHIFT>(d, s, st);
 }
 
 template <class T>

@@ -53,24 +53,34 @@ __device__ inline void hold(V &v) {
   }
 }
 
-// `n` (clamped) of the 8 elements at column c of a row, zeros in the place of the others (a row that
-// all lanes share is a scalar base, and c a 32-bit offset from it). Matrices pass through
-// once: nontemporal (a 4096 x 8192 norm of bf16 56 us against 65, a checkpoint of 8192 x 16384 71
-// against 90); what is read again soon is loaded and stored with `again`. A row's last elements
-// come in pieces of 1, 2 and 4 from its end, each moving up what it precedes: three branches that
-// only the row's last lane takes.
+// How the last vector of a row is loaded. FULL: cols is a multiple of 8, so there is none of fewer
+// than 8 elements. SHIFT (cols >= 8): every lane loads 8 elements that lie in the row, the last ones
+// from cols - 8, and moves them into place where it uses them -- no load has a branch around it,
+// whose two ways would have to wait for each other's registers (a 8192 x 4099 gradient of bf16 69 us
+// against 118). PIECES: in pieces of 1, 2 and 4, where there are no 8 elements, or where the ones before
+// the row's last may have been replaced already (in place, in another wave).
+enum { FULL = 0, SHIFT = 1, PIECES = 2 };
+inline int tail_of(long cols) { return cols % 8 == 0 ? FULL : cols >= 8 ? SHIFT : PIECES; }
+
+// 8 elements at column c of a row (a row that all lanes share is a scalar base, and c a 32-bit offset
+// from it). Matrices pass through once: nontemporal (a 4096 x 8192 norm of bf16 56 us against 65, a
+// checkpoint of 8192 x 16384 71 against 90); what is read again soon is loaded with `again`.
 template <class T, bool again = false>
-__device__ inline raw8<T> load8(const T *row, unsigned c, int n) {
+__device__ inline raw8<T> load8(const T *row, unsigned c) {
+  typedef typename any<raw8<T>, sizeof(T)>::type RA;
+  const RA *p = (const RA *)((const char *)row + c * (unsigned)sizeof(T));
+  if (again) return *p;
+  return __builtin_nontemporal_load(p);
+}
+
+// n (clamped) of 8 elements, zeros behind them: pieces of 1, 2 and 4 from its end, each moving up
+// what it precedes
+template <class T>
+__device__ inline raw8<T> load_pieces(const T *row, int n) {
   constexpr int E = sizeof(T);
-  typedef raw8<T> R;
-  const char *p = (const char *)row + c * (unsigned)E;
-  if (!__builtin_constant_p(n)) asm volatile("" : "+v"(n)); // or the branches of several loads are threaded together
-  if (n >= 8) {
-    typedef typename any<R, E>::type RA;
-    if (again) return *(const RA *)p;
-    return __builtin_nontemporal_load((const RA *)p);
-  }
-  R r = (R)0u;
+  const char *p = (const char *)row;
+  if (n >= 8) return load8(row, 0u);
+  raw8<T> r = (raw8<T>)0u;
   if (n <= 0) return r;
   if constexpr (E == 4) {
     if (n & 1) r[0] = *(const unsigned *)(p + 4 * (n & 6));
@@ -81,9 +91,8 @@ __device__ inline raw8<T> load8(const T *row, unsigned c, int n) {
       r[1] = v[1];
     }
     if (n & 4) {
-      const u4 v = *(const typename any<u4, 4>::type *)p;
       r.hi = r.lo;
-      r.lo = v;
+      r.lo = *(const typename any<u4, 4>::type *)p;
     }
   } else if constexpr (E == 2) {
     if (n & 1) r[0] = *(const unsigned short *)(p + 2 * (n & 6));
@@ -106,11 +115,44 @@ __device__ inline raw8<T> load8(const T *row, unsigned c, int n) {
   return r;
 }
 
+// the last n of 8 elements (none if n <= 0) moved to the front, zeros behind them
+template <class T>
+__device__ inline raw8<T> last8(raw8<T> r, int n) {
+  constexpr int E = sizeof(T);
+  asm volatile("" : "+v"(n)); // or the branches of several vectors are threaded together
+  if (n >= 8) return r;
+  const int k = n > 0 ? 8 - n : 0;
+  if constexpr (E == 4) {
+    if (k & 4) {
+      r.lo = r.hi;
+      r.hi = (u4)0u;
+    }
+    if (k & 2) r = __builtin_shufflevector(r, (u8x)0u, 2, 3, 4, 5, 6, 7, 8, 9);
+    if (k & 1) r = __builtin_shufflevector(r, (u8x)0u, 1, 2, 3, 4, 5, 6, 7, 8);
+  } else if constexpr (E == 2) {
+    if (k & 4) {
+      r.lo = r.hi;
+      r.hi = (u2)0u;
+    }
+    if (k & 2) r = __builtin_shufflevector(r, (u4)0u, 1, 2, 3, 4);
+    if (k & 1) {
+      r[0] = __builtin_amdgcn_alignbit(r[1], r[0], 16);
+      r[1] = __builtin_amdgcn_alignbit(r[2], r[1], 16);
+      r[2] = __builtin_amdgcn_alignbit(r[3], r[2], 16);
+      r[3] >>= 16;
+    }
+  } else {
+    r = __builtin_bit_cast(u2, __builtin_bit_cast(unsigned long, r) >> 8 * k);
+  }
+  return n > 0 ? r : (raw8<T>)0u;
+}
+
+// n (clamped) of 8 elements to column c of a row
 template <class T, bool again = false>
 __device__ inline void store8(T *row, unsigned c, raw8<T> v, int n) {
   constexpr int E = sizeof(T);
   char *p = (char *)row + c * (unsigned)E;
-  if (!__builtin_constant_p(n)) asm volatile("" : "+v"(n));
+  if (!__builtin_constant_p(n)) asm volatile("" : "+v"(n)); // as in last8
   if (n >= 8) {
     typedef typename any<raw8<T>, E>::type RA;
     if (again) *(RA *)p = v;

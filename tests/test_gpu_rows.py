@@ -298,6 +298,11 @@ def test_act_at_its_ends(kind):
     assert bool((h[0, 9::2] == 0).all()) and bool((h[0, 5::2] <= 0).all())
     v, _, bv, _ = ref.act(kind, a[:, :8])
     ref.close(h[:, :8], v, bv)
+    x = torch.tensor([[math.inf, math.nan, 1.0]], device="cuda")
+    for t in ref.TYPES.values():
+        xt, ht = x.to(t), torch.empty_like(x.to(t))
+        go(emac.act_init(1, 3, CODE[t], KINDS[kind], xt.data_ptr(), ht.data_ptr()))
+        assert float(ht[0, 0]) == math.inf and math.isnan(float(ht[0, 1])) and 0.7 < float(ht[0, 2]) < 0.9
     da, dh = torch.empty_like(a), torch.ones_like(a)
     for j in range(16):  # each value a block of its own, restored to within a rounding
         q, s = torch.full((1, 1), 127 if a[0, j] > 0 else -127, dtype=torch.int8, device="cuda"), (a[:, j:j + 1].abs() / 127).contiguous()
@@ -343,6 +348,35 @@ def test_in_place():
     go(emac.act_grad_init(rows, cols, emac.BF16, emac.GELU, src.data_ptr(), q.data_ptr(), sc.data_ptr(), da.data_ptr()),
        emac.act_grad_init(rows, cols, emac.BF16, emac.GELU, dh2.data_ptr(), q.data_ptr(), sc.data_ptr(), dh2.data_ptr()))
     assert torch.equal(da, dh2)
+
+
+@pytest.mark.parametrize("cols", [9, 129, 130, 519, 521, 1031, 4097, 8193])
+def test_in_place_at_odd_widths(cols):
+    """In place where the row's last vector is not whole and may lie in another wave than the one before."""
+    rows, gen = 500, rnd(cols)
+    a, b, dh, res = (torch.randn(rows, cols, device="cuda", generator=gen).bfloat16() for _ in range(4))
+    nb = -(-cols // 128)
+    q, q2, q3 = (torch.empty(rows, cols, dtype=torch.int8, device="cuda") for _ in range(3))
+    s, s2, s3 = (torch.empty(rows, nb, device="cuda") for _ in range(3))
+    h, da, db = torch.empty_like(a), torch.empty_like(a), torch.empty_like(a)
+    code, silu = emac.BF16, emac.SILU
+    go(emac.act_init(rows, cols, code, silu, a.data_ptr(), h.data_ptr(), b=b.data_ptr(), qa=q.data_ptr(), sa=s.data_ptr(), qb=q2.data_ptr(), sb=s2.data_ptr()),
+       emac.act_grad_init(rows, cols, code, silu, dh.data_ptr(), q.data_ptr(), s.data_ptr(), da.data_ptr(), qb=q2.data_ptr(), sb=s2.data_ptr(), db=db.data_ptr()))
+    a2, dh2, db2 = a.clone(), dh.clone(), torch.empty_like(a)
+    go(emac.act_init(rows, cols, code, silu, a2.data_ptr(), a2.data_ptr(), b=b.data_ptr(), qa=q3.data_ptr(), sa=s3.data_ptr(), qb=q2.data_ptr(), sb=s2.data_ptr()),
+       emac.act_grad_init(rows, cols, code, silu, dh2.data_ptr(), q.data_ptr(), s.data_ptr(), dh2.data_ptr(), qb=q2.data_ptr(), sb=s2.data_ptr(), db=db2.data_ptr()))
+    assert torch.equal(a2, h) and torch.equal(q3, q) and torch.equal(s3, s) and torch.equal(dh2, da) and torch.equal(db2, db)
+    x, res2, mean, rstd, y = torch.empty_like(a), res.clone(), torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda"), torch.empty_like(a)
+    go(emac.layernorm_init(rows, cols, code, [a.data_ptr()], y.data_ptr(), residual=res.data_ptr(), sum=x.data_ptr(), mean=mean.data_ptr(), rstd=rstd.data_ptr()),
+       emac.layernorm_init(rows, cols, code, [a.data_ptr()], residual=res2.data_ptr(), sum=res2.data_ptr()))
+    assert torch.equal(x, ref.fold([a], res)) and torch.equal(res2, x)
+    y2, dx, dy2, dw, dw2 = a.clone(), torch.empty_like(a), dh.clone(), torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+    go(emac.layernorm_init(rows, cols, code, [y2.data_ptr()], y2.data_ptr(), residual=res.data_ptr()))
+    assert torch.equal(y2, y)
+    for g, o, w in ((dh, dx, dw), (dy2, dy2, dw2)):
+        go(emac.layernorm_grad_init(rows, cols, code, [g.data_ptr()], mean.data_ptr(), rstd.data_ptr(), x=x.data_ptr(), dx=o.data_ptr(), dsum=g.data_ptr(),
+                                    dweight=w.data_ptr(), gdtype=emac.FLOAT))
+    assert torch.equal(dy2, dx) and torch.equal(dw2, dw)
 
 
 def test_in_place_wide_gradient():
