@@ -34,30 +34,55 @@ struct lanes {
   }
 };
 
-// A lane's vector i of a row. A lane past the row's end loads the row's last vector again: with
-// SHIFT that is zeros once moved into place, with FULL it is kept out of every sum and store.
+// A lane's vector i of a row. A lane past the row's end loads the row's last 8 elements and keeps
+// them out of every sum and store.
 template <int TAIL>
 struct slot {
-  int own, c, n; // first column, the column loaded from, elements (0 or less: none)
+  int own, c, n; // first column of its own, of those it loads; its own elements (0 or less: none)
   __device__ slot(int i, int per, int l, int cols, bool live) {
     own = (l + i * per) * 8;
     n = live ? cols - own : 0;
-    c = min(own, cols - 8);
+    c = TAIL != PIECES ? min(own, cols - 8) : own;
   }
   __device__ bool in() const { return n > 0; }
+  // whether the lane's element j is its own
+  __device__ bool mine(int j) const { return TAIL == WHOLE ? j >= 8 - n : j < n; }
   template <class T, bool again = false>
-  __device__ raw8<T> load(const void *row) const { // to be put() where it is used
-    if constexpr (TAIL == PIECES) return load_pieces((const T *)row + own, n);
-    else return load8<T, again>((const T *)row, (unsigned)c);
+  __device__ raw8<T> load(const void *row) const {
+    if constexpr (TAIL != PIECES) return load8<T, again>((const T *)row, (unsigned)c);
+    else return load_pieces((const T *)row + c, n);
   }
+  // what was loaded, where it is used
   template <class T>
   __device__ raw8<T> put(raw8<T> v) const {
     if constexpr (TAIL == SHIFT) return last8<T>(v, n);
     else return v;
   }
-  template <class T>
+  __device__ f8 put(f8 v) const {
+    if constexpr (TAIL == SHIFT) return __builtin_bit_cast(f8, last8<float>(__builtin_bit_cast(u8x, v), n));
+    else return v;
+  }
+  template <class T, bool again = false>
   __device__ void store(void *row, raw8<T> v) const {
-    if (in()) store8<T>((T *)row, (unsigned)own, v, TAIL == FULL ? 8 : n);
+    if (in()) store8<T, again>((T *)row, (unsigned)(TAIL == WHOLE ? c : own), v, TAIL == WHOLE ? 8 : n);
+  }
+  // the sum of f's, and of f h's, own elements
+  __device__ void sums(f8 f, f8 h, float &s0, float &s1) const {
+    int m = n;
+    asm volatile("" : "+v"(m)); // or the branches of several vectors are threaded together, and their registers
+    if (m >= 8) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        s0 += f[j];
+        s1 += f[j] * h[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        s0 += mine(j) ? f[j] : 0.0f;
+        s1 += mine(j) ? f[j] * h[j] : 0.0f;
+      }
+    }
   }
 };
 template <class T>
@@ -109,18 +134,19 @@ __device__ inline f8 fold8(const void *const *src, int nsrc, long row, long stri
       if (t0 + k < nsrc) raw[k] = at.template load<T>(row_of<T>(src[t0 + k], row, stride));
 #pragma unroll
     for (int k = 0; k < B; k++)
-      if (t0 + k < nsrc) s = t0 + k ? s + widen<T>(at.template put<T>(raw[k])) : widen<T>(at.template put<T>(raw[k]));
+      if (t0 + k < nsrc) s = t0 + k ? s + widen<T>(raw[k]) : widen<T>(raw[k]);
   }
   return s;
 }
 
-// A row's weights (`none` without any), in registers over all rows of a workgroup: as floats at up
-// to two vectors to a lane, else (AHEAD) as loaded. A load of them among the next row's would be worse
-// than its own latency: loads return in order, so waiting for it is waiting for the next row. Only the
-// forms that do not load ahead load them at their use. ZERO: zeros past the row's end.
-template <class W, int NV, int TAIL, bool ZERO, bool AHEAD>
+// A row's weights (`none` without any), in registers over all rows of a workgroup. A load of them
+// among the next row's would be worse than its own latency: loads return in order, so waiting for it
+// is waiting for the next row. At up to two vectors to a lane they are held as floats; as loaded at
+// more, and by the forms that do not load ahead, which would wait for them before their first row's
+// loads. The widest of those load them at their use.
+template <class W, int NV, int TAIL, bool AHEAD>
 struct weights {
-  static constexpr bool kFloats = NV <= 2, kRaw = !kFloats && AHEAD;
+  static constexpr bool kFloats = NV <= 2 && AHEAD, kRaw = !kFloats && (AHEAD || NV <= 2);
   f8 v[kFloats ? NV : 1];
   raw8<W> r[kRaw ? NV : 1];
   const W *p;
@@ -134,9 +160,7 @@ struct weights {
     }
   }
   __device__ f8 floats(raw8<W> w, const slot<TAIL> &at) const {
-    f8 f = p ? widen<W>(at.template put<W>(w)) : (f8)none;
-    if (ZERO && !at.in()) f = (f8)0.0f;
-    return f;
+    return p ? widen<W>(at.template put<W>(w)) : (f8)none;
   }
   __device__ f8 at(int i, const slot<TAIL> &s) const {
     if (kFloats) return v[kFloats ? i : 0];
@@ -160,7 +184,7 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
   const float inv = 1.0f / (float)cols;
   __shared__ float red[2][8][1];
   row_sum<MODE, 1> sum_row(red);
-  const weights<W, NV, TAIL, false, AHEAD> w(d.weight, 1.0f, per, l, cols), b(d.bias, 0.0f, per, l, cols);
+  const weights<W, NV, TAIL, AHEAD> w(d.weight, 1.0f, per, l, cols), b(d.bias, 0.0f, per, l, cols);
   const long step = (long)gridDim.x * ln.kRows;
   raw8<T> nx[MULTI ? 1 : NV], nr[NV];
   const auto load = [&](long row) {
@@ -187,20 +211,19 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
       if (MULTI || d.residual) {
         f8 f;
         if (MULTI) f = fold8<T>(d.src, d.nsrc, within(row), d.src_stride, at);
-        else f = widen<T>(at.template put<T>(nx[MULTI ? 0 : i]));
-        if (d.residual) f += widen<T>(at.template put<T>(nr[i]));
+        else f = widen<T>(nx[MULTI ? 0 : i]);
+        if (d.residual) f += widen<T>(nr[i]);
         x[i] = round_to<T>(f);
       } else {
-        x[i] = at.template put<T>(nx[MULTI ? 0 : i]);
+        x[i] = nx[MULTI ? 0 : i];
       }
-      if (TAIL == FULL && !at.in()) x[i] = (raw8<T>)0u;
+      x[i] = at.template put<T>(x[i]);
     }
     if (AHEAD) load(within(row + step));
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const f8 f = widen<T>(x[i]);
-#pragma unroll
-      for (int j = 0; j < 8; j++) s[0] += f[j];
+      float none = 0.0f;
+      slot<TAIL>(i, per, l, cols, true).sums(widen<T>(x[i]), (f8)0.0f, s[0], none);
     }
     if (d.y || d.mean || d.rstd) {
       sum_row(s);
@@ -210,10 +233,8 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
       for (int i = 0; i < NV; i++) {
         const slot<TAIL> at(i, per, l, cols, true);
         const f8 f = widen<T>(x[i]) - mean;
-        float t = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) t += TAIL == FULL || j < at.n ? f[j] * f[j] : 0.0f;
-        s[0] += at.in() ? t : 0.0f;
+        float none = 0.0f;
+        at.sums(f * f, (f8)0.0f, s[0], none);
       }
       sum_row(s);
       const float rstd = 1.0f / sqrtf(s[0] * inv + (float)d.eps);
@@ -228,14 +249,14 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
         const f8 f = (widen<T>(x[i]) - mean) * rstd * w.at(i, at) + b.at(i, at);
         at.template store<T>((T *)d.y + row * d.y_stride, round_to<T>(f));
       }
-    } else if (MODE == 0 && TAIL == SHIFT) {
+    } else if (MODE == 0 && TAIL != PIECES) {
       __syncthreads(); // sum may replace the residual: the row's last lane has read what the one before it owns
     }
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       const slot<TAIL> at(i, per, l, cols, live);
       if (d.sum) at.template store<T>((T *)d.sum + row * d.sum_stride, x[i]);
-      if (d.q) { // every lane of a block takes part; lanes past the row hold zeros
+      if (d.q) { // every lane of a block takes part; what a lane holds of another's is of the same block
         const block8 k = quantise<T>(x[i]);
         at.template store<signed char>(d.q + row * d.q_stride, k.q);
         if (at.in() && at.own % EMAC_BLOCK8 == 0) d.scale[row * nblk + at.own / EMAC_BLOCK8] = k.scale;
@@ -258,22 +279,21 @@ __device__ inline void put_grad(void *out, int gdtype, int accumulate, long c, f
   }
 }
 
-// Column sums that a workgroup has finished, 8 of each at column c, into its partial row, or (no
-// partial rows) into the gradients
-__device__ inline void put_cols(const ext_mpi_amd_layernorm_grad &d, float *part, int slice, int c, f8 w, f8 b) {
-  const int cols = (int)d.cols, n = cols - c;
-  if (n <= 0) return;
+// Column sums that a workgroup has finished, 8 of each, into its partial row, or (no partial rows)
+// into the gradients
+template <int TAIL>
+__device__ inline void put_cols(const ext_mpi_amd_layernorm_grad &d, float *part, int slice, const slot<TAIL> &at, f8 w, f8 b) {
   if (part) {
-    float *p = part + (long)slice * 2 * cols;
-    store8<float, true>(p, c, round_to<float>(w), n);
-    store8<float, true>(p + cols, c, round_to<float>(b), n);
+    float *p = part + (long)slice * 2 * d.cols;
+    at.template store<float, true>(p, round_to<float>(w));
+    at.template store<float, true>(p + d.cols, round_to<float>(b));
     return;
   }
 #pragma unroll
   for (int j = 0; j < 8; j++)
-    if (j < n) {
-      if (d.dweight) put_grad(d.dweight, d.gdtype, d.accumulate, c + j, w[j]);
-      if (d.dbias) put_grad(d.dbias, d.gdtype, d.accumulate, c + j, b[j]);
+    if (at.mine(j)) {
+      if (d.dweight) put_grad(d.dweight, d.gdtype, d.accumulate, at.c + j, w[j]);
+      if (d.dbias) put_grad(d.dbias, d.gdtype, d.accumulate, at.c + j, b[j]);
     }
 }
 
@@ -309,15 +329,14 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
   constexpr bool AHEAD = !MULTI && NV <= 2;
   // y has kernels of its own (the ones for any number of leaves and any width): a load of the bias
   // among the next row's, even where no y is asked for, makes every row wait for the next
-  constexpr bool Y = MULTI && TAIL != FULL;
+  constexpr bool Y = MULTI;
   const lanes<MODE> ln;
   const int l = ln.l, per = ln.per, cols = (int)d.cols;
   const int nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
   const float inv = 1.0f / (float)cols;
   __shared__ float red[2][8][2];
   row_sum<MODE, 2> sum_row(red);
-  // zeros past the row's end: what a lane there loads enters no sum of the row
-  const weights<W, NV, TAIL, true, AHEAD> w(d.weight, 1.0f, per, l, cols);
+  const weights<W, NV, TAIL, AHEAD> w(d.weight, 1.0f, per, l, cols);
   const long step = (long)blocks * ln.kRows;
   const bool more = d.dsum && d.dx;
   f8 aw[ACC ? NV : 1] = {}, ab[ACC ? NV : 1] = {};
@@ -350,7 +369,8 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
     for (int i = 0; i < NV; i++) {
       const slot<TAIL> at(i, per, l, cols, true);
       if (MULTI) g[i] = fold8<T>(d.dy, d.nsrc, within(row), d.dy_stride, at);
-      else g[i] = widen<T>(at.template put<T>(ng[MULTI ? 0 : i]));
+      else g[i] = widen<T>(ng[MULTI ? 0 : i]);
+      g[i] = at.put(g[i]);
       if (MODE != 0 && !live) g[i] = (f8)0.0f; // a row past the last
       xh[i] = nx[i].normed(rstd, shift, at);
       dsum[i] = nd[i];
@@ -370,11 +390,7 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
         at.template store<T>((T *)d.y + row * d.y_stride, round_to<T>(y));
       }
       g[i] *= ww;
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        s[0] += g[i][j];
-        s[1] += g[i][j] * xh[i][j];
-      }
+      at.sums(g[i], xh[i], s[0], s[1]);
     }
     if (!d.dx) continue;
     sum_row(s);
@@ -413,7 +429,7 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
       if (ln.sub) return;
     }
 #pragma unroll
-    for (int i = 0; i < NV; i++) put_cols(d, part, block, (l + i * per) * 8, aw[i], ab[i]);
+    for (int i = 0; i < NV; i++) put_cols(d, part, block, slot<TAIL>(i, per, l, cols, true), aw[i], ab[i]);
   }
 }
 
@@ -440,21 +456,23 @@ __device__ inline void cols_tile(const ext_mpi_amd_layernorm_grad &d, int tile, 
     const float rstd = d.rstd[row], mean = d.mean[row];
     f8 g;
     if (MULTI) g = fold8<T>(d.dy, d.nsrc, row, d.dy_stride, at);
-    else g = widen<T>(at.template put<T>(at.template load<T>(row_of<T>(d.dy[0], row, d.dy_stride))));
+    else g = widen<T>(at.template load<T>(row_of<T>(d.dy[0], row, d.dy_stride)));
     aw += g * x.normed(rstd, -mean * rstd, at);
     ab += g;
   }
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    comb[0][k0][8 * l + j] = aw[j];
-    comb[1][k0][8 * l + j] = ab[j];
-  }
+  for (int j = 0; j < 8; j++)
+    if (at.mine(j)) {
+      comb[0][k0][at.c - tile * C + j] = aw[j];
+      comb[1][k0][at.c - tile * C + j] = ab[j];
+    }
   __syncthreads();
   for (int o = threadIdx.x; o < 2 * C; o += blockDim.x) {
     const int which = o / C, c = o % C, col = tile * C + c;
     if (col >= cols) continue;
     float s = 0.0f;
-    for (int k = 0; k < R; k++) s += comb[which][k][c];
+    for (int k = 0; k < R; k += 4) // R is a multiple of 4
+      s += (comb[which][k][c] + comb[which][k + 1][c]) + (comb[which][k + 2][c] + comb[which][k + 3][c]);
     void *out = which ? d.dbias : d.dweight;
     if (part) part[(long)slice * 2 * cols + (long)which * cols + col] = s;
     else if (out) put_grad(out, d.gdtype, d.accumulate, col, s);
@@ -465,7 +483,7 @@ __device__ inline void cols_tile(const ext_mpi_amd_layernorm_grad &d, int tile, 
 // grid: slices (x), column tiles (y).
 template <class T, bool Q8>
 __global__ __launch_bounds__(256) void layernorm_cols_kernel(const ext_mpi_amd_layernorm_grad d, float *part) {
-  cols_tile<T, 64, Q8, true, SHIFT>(d, blockIdx.y, blockIdx.x, gridDim.x, part);
+  cols_tile<T, 64, Q8, true, WHOLE>(d, blockIdx.y, blockIdx.x, gridDim.x, part);
 }
 
 // Rows without column sums, and in the workgroups behind theirs (from `blocks` on) the column sums of
@@ -474,8 +492,9 @@ template <class T, class W, int MODE, int NV, bool Q8, int TAIL>
 __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void layernorm_grad_apart_kernel(
     const ext_mpi_amd_layernorm_grad d, int blocks) {
   if ((int)blockIdx.x < blocks) grad_rows<T, W, MODE, NV, Q8, true, TAIL, false>(d, blockIdx.x, blocks, nullptr);
-  else if (TAIL == SHIFT && d.nsrc == 1 && d.cols % 8 == 0) cols_tile<T, 8, Q8, false, FULL>(d, blockIdx.x - blocks, 0, 1, nullptr);
-  else cols_tile<T, 8, Q8, true, TAIL>(d, blockIdx.x - blocks, 0, 1, nullptr);
+  else if (TAIL == PIECES) cols_tile<T, 8, Q8, true, PIECES>(d, blockIdx.x - blocks, 0, 1, nullptr);
+  else if (d.nsrc == 1) cols_tile<T, 8, Q8, false, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr);
+  else cols_tile<T, 8, Q8, true, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr);
 }
 
 // ---- launches ----
@@ -495,11 +514,20 @@ inline row_shape row_shape_of(long cols) {
   return s;
 }
 
+// Workgroups to a CU, as few as keep enough loads in flight: 8 KB of rows of each matrix (65536 x 256
+// bf16 norm: 2 to a CU, 4 KB, 35 us, 4 27 us; 65536 x 512: 2, 8 KB, 46 us, 4 50 us), and 8 waves. More
+// of them cost more than they hide, the gradient the most: each leaves a partial row.
+inline int per_cu(const row_shape &s, long cols, int dtype, bool most) {
+  const long bytes = (s.mode ? 256 / s.mode : 1) * cols * (dtype == EXT_MPI_AMD_FLOAT ? 4 : 2);
+  const long by_bytes = (8192 + bytes / 2) / bytes, by_waves = most ? (512 + s.block - 1) / s.block : s.block > 256 ? 1 : 512 / s.block;
+  return (int)(by_bytes > 5 ? 5 : by_bytes > by_waves ? by_bytes : by_waves);
+}
+
 template <class T, class W, int MODE, int NV, bool MULTI, int TAIL>
 int norm_go(const ext_mpi_amd_layernorm &d, const row_shape &s, hipStream_t st) {
   constexpr int rows = lanes<MODE>::kRows;
   const long want = (d.rows + rows - 1) / rows;
-  const long most = (long)EMAC_NORM_CUS * ((512 + s.block - 1) / s.block); // 8 waves to a CU, or a few more
+  const long most = (long)EMAC_NORM_CUS * per_cu(s, d.cols, d.dtype, true);
   const int grid = (int)(want < most ? want : most);
   layernorm_kernel<T, W, MODE, NV, MULTI, TAIL><<<grid, s.block, 0, st>>>(d);
   return launched();
@@ -507,23 +535,24 @@ int norm_go(const ext_mpi_amd_layernorm &d, const row_shape &s, hipStream_t st) 
 
 template <class T, class W, int MODE, int NV>
 int norm_nv(const ext_mpi_amd_layernorm &d, const row_shape &s, hipStream_t st) {
-  const bool full = d.cols % 8 == 0;
-  if (d.nsrc > 1) return full ? norm_go<T, W, MODE, NV, true, FULL>(d, s, st) : norm_go<T, W, MODE, NV, true, SHIFT>(d, s, st);
-  return full ? norm_go<T, W, MODE, NV, false, FULL>(d, s, st) : norm_go<T, W, MODE, NV, false, SHIFT>(d, s, st);
+  if (tail_of(d.cols, d.q) == SHIFT) return norm_go<T, W, MODE, NV, true, SHIFT>(d, s, st);
+  if (d.nsrc > 1) return norm_go<T, W, MODE, NV, true, WHOLE>(d, s, st);
+  return norm_go<T, W, MODE, NV, false, WHOLE>(d, s, st);
 }
 
 template <class T, class W>
 int norm_w(const ext_mpi_amd_layernorm &d, hipStream_t st) {
   const row_shape s = row_shape_of(d.cols);
-  if (tail_of(d.cols) == PIECES) return norm_go<T, W, 16, 1, true, PIECES>(d, s, st);
+  const int tail = tail_of(d.cols, d.q);
+  if (tail == PIECES) return norm_go<T, W, 16, 1, true, PIECES>(d, s, st);
   if (s.mode == 16) return norm_nv<T, W, 16, 1>(d, s, st);
   if (s.mode == 64) return norm_nv<T, W, 64, 1>(d, s, st);
   if (s.nv == 1) return norm_nv<T, W, 0, 1>(d, s, st);
   if (s.nv == 2) return norm_nv<T, W, 0, 2>(d, s, st);
   if (s.nv == 4) return norm_nv<T, W, 0, 4>(d, s, st);
-  // wider: the forms that take any number of leaves and any width
-  if (s.nv == 8) return norm_go<T, W, 0, 8, true, SHIFT>(d, s, st);
-  return norm_go<T, W, 0, 16, true, SHIFT>(d, s, st);
+  // wider: the forms that take any number of leaves
+  if (s.nv == 8) return tail == WHOLE ? norm_go<T, W, 0, 8, true, WHOLE>(d, s, st) : norm_go<T, W, 0, 8, true, SHIFT>(d, s, st);
+  return tail == WHOLE ? norm_go<T, W, 0, 16, true, WHOLE>(d, s, st) : norm_go<T, W, 0, 16, true, SHIFT>(d, s, st);
 }
 
 // the gradient's launch: `grid` workgroups take the rows, and each leaves a partial row of column
@@ -551,7 +580,7 @@ inline grad_shape grad_shape_of(const ext_mpi_amd_layernorm_grad &d) {
   s.apart = sums && d.rows <= 4 * (lanes / 8) && twice <= 16L << 20;
   s.tiles = s.apart ? (int)((d.cols + 63) / 64) : 0;
   if (s.apart) s.r.block = lanes;
-  const long most = s.apart ? 2048 : (long)EMAC_NORM_CUS * (s.r.block > 256 ? 1 : 512 / s.r.block); // 8 waves to a CU, or a few fewer
+  const long most = s.apart ? 2048 : (long)EMAC_NORM_CUS * per_cu(s.r, d.cols, d.dtype, false);
   s.grid = (int)(want < most ? want : most);
   if (s.apart && !d.dx && !d.y) s.grid = 0;
   return s;
@@ -578,16 +607,17 @@ int grad_go(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *par
 
 template <class T, class W, int MODE, int NV>
 int grad_nv(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part, hipStream_t st) {
-  const bool full = d.cols % 8 == 0 && !d.y;
-  if (s.apart) return apart_go<T, W, MODE, NV, SHIFT>(d, s, st);
-  if (d.nsrc > 1 || d.y)
-    return full ? grad_go<T, W, MODE, NV, true, FULL>(d, s, part, st) : grad_go<T, W, MODE, NV, true, SHIFT>(d, s, part, st);
-  return full ? grad_go<T, W, MODE, NV, false, FULL>(d, s, part, st) : grad_go<T, W, MODE, NV, false, SHIFT>(d, s, part, st);
+  if (tail_of(d.cols, d.q) == SHIFT)
+    return s.apart ? apart_go<T, W, MODE, NV, SHIFT>(d, s, st) : grad_go<T, W, MODE, NV, true, SHIFT>(d, s, part, st);
+  if (s.apart) return apart_go<T, W, MODE, NV, WHOLE>(d, s, st);
+  if (d.nsrc > 1 || d.y) return grad_go<T, W, MODE, NV, true, WHOLE>(d, s, part, st);
+  return grad_go<T, W, MODE, NV, false, WHOLE>(d, s, part, st);
 }
 
 template <class T, class W>
 int grad_w(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part, hipStream_t st) {
-  if (tail_of(d.cols) == PIECES)
+  const int tail = tail_of(d.cols, d.q);
+  if (tail == PIECES)
     return s.apart ? apart_go<T, W, 16, 1, PIECES>(d, s, st) : grad_go<T, W, 16, 1, true, PIECES>(d, s, part, st);
   if (s.r.mode == 16) return grad_nv<T, W, 16, 1>(d, s, part, st);
   if (s.r.mode == 64) return grad_nv<T, W, 64, 1>(d, s, part, st);
@@ -595,8 +625,8 @@ int grad_w(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part
   if (s.r.nv == 2) return grad_nv<T, W, 0, 2>(d, s, part, st);
   if (s.r.nv == 4) return grad_nv<T, W, 0, 4>(d, s, part, st);
   // wide: the rows alone (the column sums, if any, have a launch of their own before this one)
-  if (s.r.nv == 8) return apart_go<T, W, 0, 8, SHIFT>(d, s, st);
-  return apart_go<T, W, 0, 16, SHIFT>(d, s, st);
+  if (s.r.nv == 8) return tail == WHOLE ? apart_go<T, W, 0, 8, WHOLE>(d, s, st) : apart_go<T, W, 0, 8, SHIFT>(d, s, st);
+  return tail == WHOLE ? apart_go<T, W, 0, 16, WHOLE>(d, s, st) : apart_go<T, W, 0, 16, SHIFT>(d, s, st);
 }
 
 template <class T>

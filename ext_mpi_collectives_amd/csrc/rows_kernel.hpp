@@ -53,14 +53,18 @@ __device__ inline void hold(V &v) {
   }
 }
 
-// How the last vector of a row is loaded. FULL: cols is a multiple of 8, so there is none of fewer
-// than 8 elements. SHIFT (cols >= 8): every lane loads 8 elements that lie in the row, the last ones
-// from cols - 8, and moves them into place where it uses them -- no load has a branch around it,
-// whose two ways would have to wait for each other's registers (a 8192 x 4099 gradient of bf16 69 us
-// against 118). PIECES: in pieces of 1, 2 and 4, where there are no 8 elements, or where the ones before
-// the row's last may have been replaced already (in place, in another wave).
-enum { FULL = 0, SHIFT = 1, PIECES = 2 };
-inline int tail_of(long cols) { return cols % 8 == 0 ? FULL : cols >= 8 ? SHIFT : PIECES; }
+// How a row's last vector of n < 8 elements is taken. WHOLE (cols >= 8): its lane takes 8 elements
+// like every other, the row's last, of which its own are the last n: it keeps the others out of sums,
+// and stores them too, as the same bits that the lane before it stores. No load or store has a branch
+// around it, and no two ways of one that would have to wait for each other's registers (a 8192 x 4099
+// gradient of bf16 72 us against 118). SHIFT: loaded like that, but its own elements moved to the front
+// where they are used, and stored alone: where a checkpoint's last block has fewer than 8 columns, so
+// that the others have another scale. PIECES: its n elements alone, in pieces of 1, 2 and 4, where there
+// are no 8, or where the others may have been replaced already (in place, in another wave).
+enum { WHOLE = 0, SHIFT = 1, PIECES = 2 };
+inline int tail_of(long cols, bool saved) {
+  return cols < 8 ? PIECES : saved && cols % EMAC_BLOCK8 > 0 && cols % EMAC_BLOCK8 < 8 ? SHIFT : WHOLE;
+}
 
 // 8 elements at column c of a row (a row that all lanes share is a scalar base, and c a 32-bit offset
 // from it). Matrices pass through once: nontemporal (a 4096 x 8192 norm of bf16 56 us against 65, a
@@ -119,7 +123,7 @@ __device__ inline raw8<T> load_pieces(const T *row, int n) {
 template <class T>
 __device__ inline raw8<T> last8(raw8<T> r, int n) {
   constexpr int E = sizeof(T);
-  asm volatile("" : "+v"(n)); // or the branches of several vectors are threaded together
+  asm volatile("" : "+v"(n)); // as in slot::sums
   if (n >= 8) return r;
   const int k = n > 0 ? 8 - n : 0;
   if constexpr (E == 4) {
@@ -147,12 +151,12 @@ __device__ inline raw8<T> last8(raw8<T> r, int n) {
   return n > 0 ? r : (raw8<T>)0u;
 }
 
-// n (clamped) of 8 elements to column c of a row
+// the first n (clamped) of 8 elements to column c of a row
 template <class T, bool again = false>
 __device__ inline void store8(T *row, unsigned c, raw8<T> v, int n) {
   constexpr int E = sizeof(T);
   char *p = (char *)row + c * (unsigned)E;
-  if (!__builtin_constant_p(n)) asm volatile("" : "+v"(n)); // as in last8
+  if (!__builtin_constant_p(n)) asm volatile("" : "+v"(n)); // as in slot::sums
   if (n >= 8) {
     typedef typename any<raw8<T>, E>::type RA;
     if (again) *(RA *)p = v;
