@@ -16,20 +16,23 @@
 
 namespace emac_rows {
 
-// How the lanes of a workgroup share out rows: MODE 16 or 64 lanes to a row, 256 lanes in all, or
-// (MODE 0) all of a workgroup of as many waves as the row needs at NV vectors to a lane, at most 8.
-// Few waves with many registers (up to 256) and the next row's loads in flight hide the latency; more
-// waves only repeat what every wave does once a row.
+// How the lanes of a workgroup share out rows: MODE 16 or 64 lanes to a row, 256 lanes in all, or all
+// of a workgroup of as many waves as the row needs at NV vectors to a lane, at most 8 (MODE 512) or 16
+// (MODE 1024). With many rows, few waves with many registers (up to 256) and the next row's loads in
+// flight hide the latency; more waves only repeat what every wave does once a row. With a row or less
+// for each CU they shorten it: 32 rows of 8192 bf16 from 8 leaves 7.4 us with 16 waves, 7.8 with 8.
 template <int MODE>
 struct lanes {
-  static constexpr int kBlock = MODE ? 256 : 512; // at most
-  static constexpr int kWaves = MODE ? 4 : 2;     // waves to a SIMD that the registers allow
-  static constexpr int kRows = MODE ? 256 / MODE : 1;
+  static constexpr bool kOneRow = MODE >= 512;             // a workgroup takes one row at a time
+  static constexpr int kBlock = kOneRow ? MODE : 256;      // at most
+  static constexpr int kWaves = MODE == 512 ? 2 : 4;       // waves to a SIMD that the registers allow
+  static constexpr int kRows = kOneRow ? 1 : 256 / MODE;
+  static constexpr int kSlots = MODE == 1024 ? 16 : 8;     // waves that share a row, at most
   int per, l, sub; // lanes to a row, this lane's place in it, its row in the workgroup
   __device__ lanes() {
-    per = MODE ? MODE : (int)blockDim.x;
-    l = MODE ? threadIdx.x % (MODE ? MODE : 1) : threadIdx.x;
-    sub = MODE ? threadIdx.x / (MODE ? MODE : 1) : 0;
+    per = kOneRow ? (int)blockDim.x : MODE;
+    l = kOneRow ? threadIdx.x : threadIdx.x % MODE;
+    sub = kOneRow ? 0 : threadIdx.x / MODE;
     if (MODE == 64) sub = __builtin_amdgcn_readfirstlane(sub);
   }
 };
@@ -91,52 +94,63 @@ __device__ inline const T *row_of(const void *p, long row, long stride) {
 }
 
 // Sums over a row's lanes. Between waves they go through LDS: each wave leaves its own, and after
-// one barrier 8 lanes of every wave add the up to 8 of them; the two slots are used in turn, so
+// one barrier 8 or 16 lanes of every wave add as many of them; the two slots are used in turn, so
 // a slot's last read and its next write have a barrier between them.
 template <int MODE, int NS>
 struct row_sum {
-  float (*red)[8][NS];
+  static constexpr int kSlots = lanes<MODE>::kSlots;
+  float (*red)[kSlots][NS];
   int turn;
-  __device__ row_sum(float (*r)[8][NS]) : red(r), turn(0) {
-    if (MODE == 0) { // the places of waves that are not there
+  __device__ row_sum(float (*r)[kSlots][NS]) : red(r), turn(0) {
+    if (lanes<MODE>::kOneRow) { // the places of waves that are not there
       const int nw = blockDim.x / 64, t = threadIdx.x;
-      if (t < 16 && t % 8 >= nw) {
+      if (t < 2 * kSlots && t % kSlots >= nw) {
 #pragma unroll
-        for (int k = 0; k < NS; k++) r[t / 8][t % 8][k] = 0.0f;
+        for (int k = 0; k < NS; k++) r[t / kSlots][t % kSlots][k] = 0.0f;
       }
     }
   }
   __device__ void operator()(float (&v)[NS]) {
 #pragma unroll
     for (int k = 0; k < NS; k++) v[k] = MODE == 16 ? sum16(v[k]) : sum64(v[k]);
-    if constexpr (MODE == 0) {
+    if constexpr (lanes<MODE>::kOneRow) {
       if (threadIdx.x % 64 == 0) {
 #pragma unroll
         for (int k = 0; k < NS; k++) red[turn][threadIdx.x / 64][k] = v[k];
       }
       __syncthreads();
 #pragma unroll
-      for (int k = 0; k < NS; k++) v[k] = sum8(red[turn][threadIdx.x % 8][k]);
+      for (int k = 0; k < NS; k++) {
+        const float t = red[turn][threadIdx.x % kSlots][k];
+        v[k] = kSlots == 8 ? sum8(t) : sum16(t);
+      }
       turn ^= 1;
     }
   }
 };
 
-// ((leaf 0 + leaf 1) + ...) of 8 elements in 32 bits, the loads of a batch in flight together
-template <class T, int TAIL>
-__device__ inline f8 fold8(const void *const *src, int nsrc, long row, long stride, const slot<TAIL> &at) {
-  constexpr int B = sizeof(T) == 2 ? 8 : 4;
-  f8 s = {};
+// ((leaf 0 + leaf 1) + ...) of a lane's NV vectors of a row, in 32 bits. The loads of a batch of leaves
+// are in flight together, for all vectors: as many as 32 registers hold, 64 with several vectors (one
+// row of 8832 floats from 4 leaves 6.7 us against 10.3 vector by vector).
+template <class T, int NV, int TAIL>
+__device__ inline void fold_rows(f8 (&s)[NV], const void *const *src, int nsrc, long row, long stride, int per, int l, int cols) {
+  constexpr int fit = (NV == 1 ? 16 : 32) / (NV * (int)sizeof(T)), B = fit < 1 ? 1 : fit;
   for (int t0 = 0; t0 < nsrc; t0 += B) {
-    raw8<T> raw[B];
+    raw8<T> raw[B][NV];
 #pragma unroll
     for (int k = 0; k < B; k++)
-      if (t0 + k < nsrc) raw[k] = at.template load<T>(row_of<T>(src[t0 + k], row, stride));
+      if (t0 + k < nsrc) {
+        const T *p = row_of<T>(src[t0 + k], row, stride);
+#pragma unroll
+        for (int i = 0; i < NV; i++) raw[k][i] = slot<TAIL>(i, per, l, cols, true).template load<T>(p);
+      }
 #pragma unroll
     for (int k = 0; k < B; k++)
-      if (t0 + k < nsrc) s = t0 + k ? s + widen<T>(raw[k]) : widen<T>(raw[k]);
+      if (t0 + k < nsrc) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) s[i] = t0 + k ? s[i] + widen<T>(raw[k][i]) : widen<T>(raw[k][i]);
+      }
   }
-  return s;
 }
 
 // A row's weights (`none` without any), in registers over all rows of a workgroup. A load of them
@@ -182,7 +196,7 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
   const int l = ln.l, per = ln.per, cols = (int)d.cols;
   const int nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
   const float inv = 1.0f / (float)cols;
-  __shared__ float red[2][8][1];
+  __shared__ float red[2][lanes<MODE>::kSlots][1];
   row_sum<MODE, 1> sum_row(red);
   const weights<W, NV, TAIL, AHEAD> w(d.weight, 1.0f, per, l, cols), b(d.bias, 0.0f, per, l, cols);
   const long step = (long)gridDim.x * ln.kRows;
@@ -201,16 +215,18 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
   if (AHEAD) load(within(r0 + ln.sub));
   for (; r0 < d.rows; r0 += step) {
     const long row = r0 + ln.sub;
-    const bool live = MODE == 0 || row < d.rows;
+    const bool live = ln.kOneRow || row < d.rows;
     raw8<T> x[NV];
     float s[1] = {0.0f};
     if (!AHEAD) load(within(row));
+    f8 sum[MULTI ? NV : 1];
+    if constexpr (MULTI) fold_rows<T, NV, TAIL>(sum, d.src, d.nsrc, within(row), d.src_stride, per, l, cols);
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       const slot<TAIL> at(i, per, l, cols, true);
       if (MULTI || d.residual) {
         f8 f;
-        if (MULTI) f = fold8<T>(d.src, d.nsrc, within(row), d.src_stride, at);
+        if (MULTI) f = sum[MULTI ? i : 0];
         else f = widen<T>(nx[MULTI ? 0 : i]);
         if (d.residual) f += widen<T>(nr[i]);
         x[i] = round_to<T>(f);
@@ -249,7 +265,7 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
         const f8 f = (widen<T>(x[i]) - mean) * rstd * w.at(i, at) + b.at(i, at);
         at.template store<T>((T *)d.y + row * d.y_stride, round_to<T>(f));
       }
-    } else if (MODE == 0 && TAIL != PIECES) {
+    } else if (ln.kOneRow && TAIL != PIECES) {
       __syncthreads(); // sum may replace the residual: the row's last lane has read what the one before it owns
     }
 #pragma unroll
@@ -334,7 +350,7 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
   const int l = ln.l, per = ln.per, cols = (int)d.cols;
   const int nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
   const float inv = 1.0f / (float)cols;
-  __shared__ float red[2][8][2];
+  __shared__ float red[2][lanes<MODE>::kSlots][2];
   row_sum<MODE, 2> sum_row(red);
   const weights<W, NV, TAIL, AHEAD> w(d.weight, 1.0f, per, l, cols);
   const long step = (long)blocks * ln.kRows;
@@ -359,19 +375,19 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
   if (AHEAD) load(within(r0 + ln.sub));
   for (; r0 < d.rows; r0 += step) {
     const long row = r0 + ln.sub;
-    const bool live = MODE == 0 || row < d.rows;
+    const bool live = ln.kOneRow || row < d.rows;
     if (!AHEAD) load(within(row));
     const float rstd = nrstd, shift = -nmean * rstd;
     f8 g[NV], xh[NV];
     raw8<T> dsum[NV];
     float s[2] = {0.0f, 0.0f};
+    if constexpr (MULTI) fold_rows<T, NV, TAIL>(g, d.dy, d.nsrc, within(row), d.dy_stride, per, l, cols);
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       const slot<TAIL> at(i, per, l, cols, true);
-      if (MULTI) g[i] = fold8<T>(d.dy, d.nsrc, within(row), d.dy_stride, at);
-      else g[i] = widen<T>(ng[MULTI ? 0 : i]);
+      if (!MULTI) g[i] = widen<T>(ng[MULTI ? 0 : i]);
       g[i] = at.put(g[i]);
-      if (MODE != 0 && !live) g[i] = (f8)0.0f; // a row past the last
+      if (!ln.kOneRow && !live) g[i] = (f8)0.0f; // a row past the last
       xh[i] = nx[i].normed(rstd, shift, at);
       dsum[i] = nd[i];
     }
@@ -406,8 +422,8 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
   }
   if constexpr (ACC) {
     if (!d.dweight && !d.dbias) return;
-    if constexpr (MODE != 0) { // the rows of a workgroup taken side by side, added in order
-      __shared__ f8 comb[2][(MODE ? MODE : 1) * NV];
+    if constexpr (!lanes<MODE>::kOneRow) { // the rows of a workgroup taken side by side, added in order
+      __shared__ f8 comb[2][MODE * NV];
       for (int k = 1; k < ln.kRows; k++) {
         __syncthreads();
         if (ln.sub == k) {
@@ -454,9 +470,10 @@ __device__ inline void cols_tile(const ext_mpi_amd_layernorm_grad &d, int tile, 
     row8<T, Q8, TAIL> x;
     x.load(d, row, at, nblk);
     const float rstd = d.rstd[row], mean = d.mean[row];
-    f8 g;
-    if (MULTI) g = fold8<T>(d.dy, d.nsrc, row, d.dy_stride, at);
-    else g = widen<T>(at.template load<T>(row_of<T>(d.dy[0], row, d.dy_stride)));
+    f8 gs[1];
+    if (MULTI) fold_rows<T, 1, TAIL>(gs, d.dy, d.nsrc, row, d.dy_stride, 0, tile * LANES + l, cols);
+    else gs[0] = widen<T>(at.template load<T>(row_of<T>(d.dy[0], row, d.dy_stride)));
+    const f8 g = gs[0];
     aw += g * x.normed(rstd, -mean * rstd, at);
     ab += g;
   }
@@ -508,19 +525,20 @@ struct row_shape {
 inline row_shape row_shape_of(long cols) {
   const long v = (cols + 7) / 8; // vectors in a row
   row_shape s;
-  s.mode = v <= 16 ? 16 : v <= 64 ? 64 : 0;
-  s.nv = s.mode || v <= 512 ? 1 : v <= 1024 ? 2 : v <= 2048 ? 4 : v <= 4096 ? 8 : 16;
-  s.block = s.mode ? 256 : (int)((v + s.nv - 1) / s.nv + 63) / 64 * 64;
+  s.mode = v <= 16 ? 16 : v <= 64 ? 64 : 512;
+  s.nv = v <= 512 ? 1 : v <= 1024 ? 2 : v <= 2048 ? 4 : v <= 4096 ? 8 : 16;
+  s.block = s.mode < 512 ? 256 : (int)((v + s.nv - 1) / s.nv + 63) / 64 * 64;
   return s;
 }
 
 // Workgroups to a CU, as few as keep enough loads in flight: 8 KB of rows of each matrix (65536 x 256
 // bf16 norm: 2 to a CU, 4 KB, 35 us, 4 27 us; 65536 x 512: 2, 8 KB, 46 us, 4 50 us), and 8 waves. More
-// of them cost more than they hide, the gradient the most: each leaves a partial row.
+// of them cost more than they hide, the gradient (not `most`) above all: each leaves a partial row.
 inline int per_cu(const row_shape &s, long cols, int dtype, bool most) {
-  const long bytes = (s.mode ? 256 / s.mode : 1) * cols * (dtype == EXT_MPI_AMD_FLOAT ? 4 : 2);
+  const long bytes = (s.mode < 512 ? 256 / s.mode : 1) * cols * (dtype == EXT_MPI_AMD_FLOAT ? 4 : 2);
   const long by_bytes = (8192 + bytes / 2) / bytes, by_waves = most ? (512 + s.block - 1) / s.block : s.block > 256 ? 1 : 512 / s.block;
-  return (int)(by_bytes > 5 ? 5 : by_bytes > by_waves ? by_bytes : by_waves);
+  const long cap = most ? 8 : 5;
+  return (int)(by_bytes > cap ? cap : by_bytes > by_waves ? by_bytes : by_waves);
 }
 
 template <class T, class W, int MODE, int NV, bool MULTI, int TAIL>
@@ -542,17 +560,23 @@ int norm_nv(const ext_mpi_amd_layernorm &d, const row_shape &s, hipStream_t st) 
 
 template <class T, class W>
 int norm_w(const ext_mpi_amd_layernorm &d, hipStream_t st) {
-  const row_shape s = row_shape_of(d.cols);
+  row_shape s = row_shape_of(d.cols);
   const int tail = tail_of(d.cols, d.q);
   if (tail == PIECES) return norm_go<T, W, 16, 1, true, PIECES>(d, s, st);
+  if (s.nv == 2 && d.rows <= EMAC_NORM_CUS) { // few rows: one vector to a lane (two of them spill at 16 waves)
+    s.mode = 1024;
+    s.nv = 1;
+    s.block = (int)((d.cols + 7) / 8 + 63) / 64 * 64;
+    return tail == SHIFT ? norm_go<T, W, 1024, 1, true, SHIFT>(d, s, st) : norm_go<T, W, 1024, 1, true, WHOLE>(d, s, st);
+  }
   if (s.mode == 16) return norm_nv<T, W, 16, 1>(d, s, st);
   if (s.mode == 64) return norm_nv<T, W, 64, 1>(d, s, st);
-  if (s.nv == 1) return norm_nv<T, W, 0, 1>(d, s, st);
-  if (s.nv == 2) return norm_nv<T, W, 0, 2>(d, s, st);
-  if (s.nv == 4) return norm_nv<T, W, 0, 4>(d, s, st);
+  if (s.nv == 1) return norm_nv<T, W, 512, 1>(d, s, st);
+  if (s.nv == 2) return norm_nv<T, W, 512, 2>(d, s, st);
+  if (s.nv == 4) return norm_nv<T, W, 512, 4>(d, s, st);
   // wider: the forms that take any number of leaves
-  if (s.nv == 8) return tail == WHOLE ? norm_go<T, W, 0, 8, true, WHOLE>(d, s, st) : norm_go<T, W, 0, 8, true, SHIFT>(d, s, st);
-  return tail == WHOLE ? norm_go<T, W, 0, 16, true, WHOLE>(d, s, st) : norm_go<T, W, 0, 16, true, SHIFT>(d, s, st);
+  if (s.nv == 8) return tail == WHOLE ? norm_go<T, W, 512, 8, true, WHOLE>(d, s, st) : norm_go<T, W, 512, 8, true, SHIFT>(d, s, st);
+  return tail == WHOLE ? norm_go<T, W, 512, 16, true, WHOLE>(d, s, st) : norm_go<T, W, 512, 16, true, SHIFT>(d, s, st);
 }
 
 // the gradient's launch: `grid` workgroups take the rows, and each leaves a partial row of column
@@ -569,7 +593,7 @@ inline grad_shape grad_shape_of(const ext_mpi_amd_layernorm_grad &d) {
   s.r = row_shape_of(d.cols);
   s.wide = s.r.nv > 4;
   const bool sums = d.dweight || d.dbias;
-  const long rows = s.r.mode ? 256 / s.r.mode : 1, want = (d.rows + rows - 1) / rows;
+  const long rows = s.r.mode < 512 ? 256 / s.r.mode : 1, want = (d.rows + rows - 1) / rows;
   // few rows: the second launch, which adds the partial rows, costs more than reading the rows twice,
   // up to 4 of them to a lane (bf16, 4096 columns: 32 rows 4.5 us against 6.3, 256 rows 7.0 against
   // 10.7, 512 rows, 8 to a lane, 12.0 against 11.1)
@@ -621,12 +645,12 @@ int grad_w(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part
     return s.apart ? apart_go<T, W, 16, 1, PIECES>(d, s, st) : grad_go<T, W, 16, 1, true, PIECES>(d, s, part, st);
   if (s.r.mode == 16) return grad_nv<T, W, 16, 1>(d, s, part, st);
   if (s.r.mode == 64) return grad_nv<T, W, 64, 1>(d, s, part, st);
-  if (s.r.nv == 1) return grad_nv<T, W, 0, 1>(d, s, part, st);
-  if (s.r.nv == 2) return grad_nv<T, W, 0, 2>(d, s, part, st);
-  if (s.r.nv == 4) return grad_nv<T, W, 0, 4>(d, s, part, st);
+  if (s.r.nv == 1) return grad_nv<T, W, 512, 1>(d, s, part, st);
+  if (s.r.nv == 2) return grad_nv<T, W, 512, 2>(d, s, part, st);
+  if (s.r.nv == 4) return grad_nv<T, W, 512, 4>(d, s, part, st);
   // wide: the rows alone (the column sums, if any, have a launch of their own before this one)
-  if (s.r.nv == 8) return tail == WHOLE ? apart_go<T, W, 0, 8, WHOLE>(d, s, st) : apart_go<T, W, 0, 8, SHIFT>(d, s, st);
-  return tail == WHOLE ? apart_go<T, W, 0, 16, WHOLE>(d, s, st) : apart_go<T, W, 0, 16, SHIFT>(d, s, st);
+  if (s.r.nv == 8) return tail == WHOLE ? apart_go<T, W, 512, 8, WHOLE>(d, s, st) : apart_go<T, W, 512, 8, SHIFT>(d, s, st);
+  return tail == WHOLE ? apart_go<T, W, 512, 16, WHOLE>(d, s, st) : apart_go<T, W, 512, 16, SHIFT>(d, s, st);
 }
 
 template <class T>
