@@ -342,7 +342,7 @@ struct row8 {
 template <class T, class W, int MODE, int NV, bool Q8, bool MULTI, int TAIL, bool ACC>
 __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block, int blocks, float *part) {
   // one leaf: the next row's loads are issued before this row's sums, as far as registers go
-  constexpr bool AHEAD = !MULTI && NV <= 2;
+  constexpr bool AHEAD = !MULTI && (NV <= 2 || NV * sizeof(T) <= 6);
   // y has kernels of its own (the ones for any number of leaves and any width): a load of the bias
   // among the next row's, even where no y is asked for, makes every row wait for the next
   constexpr bool Y = MULTI;
@@ -526,7 +526,7 @@ inline row_shape row_shape_of(long cols) {
   const long v = (cols + 7) / 8; // vectors in a row
   row_shape s;
   s.mode = v <= 16 ? 16 : v <= 64 ? 64 : 512;
-  s.nv = v <= 512 ? 1 : v <= 1024 ? 2 : v <= 2048 ? 4 : v <= 4096 ? 8 : 16;
+  s.nv = v <= 512 ? 1 : v <= 1024 ? 2 : v <= 1536 ? 3 : v <= 2048 ? 4 : v <= 4096 ? 8 : 16;
   s.block = s.mode < 512 ? 256 : (int)((v + s.nv - 1) / s.nv + 63) / 64 * 64;
   return s;
 }
@@ -573,6 +573,7 @@ int norm_w(const ext_mpi_amd_layernorm &d, hipStream_t st) {
   if (s.mode == 64) return norm_nv<T, W, 64, 1>(d, s, st);
   if (s.nv == 1) return norm_nv<T, W, 512, 1>(d, s, st);
   if (s.nv == 2) return norm_nv<T, W, 512, 2>(d, s, st);
+  if (s.nv == 3) return norm_nv<T, W, 512, 3>(d, s, st);
   if (s.nv == 4) return norm_nv<T, W, 512, 4>(d, s, st);
   // wider: the forms that take any number of leaves
   if (s.nv == 8) return tail == WHOLE ? norm_go<T, W, 512, 8, true, WHOLE>(d, s, st) : norm_go<T, W, 512, 8, true, SHIFT>(d, s, st);
@@ -647,6 +648,7 @@ int grad_w(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part
   if (s.r.mode == 64) return grad_nv<T, W, 64, 1>(d, s, part, st);
   if (s.r.nv == 1) return grad_nv<T, W, 512, 1>(d, s, part, st);
   if (s.r.nv == 2) return grad_nv<T, W, 512, 2>(d, s, part, st);
+  if (s.r.nv == 3) return grad_nv<T, W, 512, 3>(d, s, part, st);
   if (s.r.nv == 4) return grad_nv<T, W, 512, 4>(d, s, part, st);
   // wide: the rows alone (the column sums, if any, have a launch of their own before this one)
   if (s.r.nv == 8) return tail == WHOLE ? apart_go<T, W, 512, 8, WHOLE>(d, s, st) : apart_go<T, W, 512, 8, SHIFT>(d, s, st);
