@@ -14,6 +14,7 @@ namespace {
 using namespace emac_rows;
 
 constexpr int kGroups = 16; // lane groups in a workgroup
+constexpr int kGridX = 23;  // a launch's lanes in one dimension stay under 2^32: from 2^23 workgroups on there are two
 
 // ---- activations: value and slope, in 32 bits ----
 // 16-bit types take the native exp2 (of x log2 e rounded) and reciprocal, 1 ulp each. Float adds what
@@ -119,7 +120,7 @@ struct span8 {
   long rows;
   int cols;
   __device__ span8(long rows_, long cols_, unsigned nblk_) : nblk(nblk_), rows(rows_), cols((int)cols_) {
-    const unsigned first = blockIdx.x * (unsigned)(U * kGroups);
+    const unsigned first = (blockIdx.y << kGridX | blockIdx.x) * (unsigned)(U * kGroups);
     row0 = first / nblk;
     blk0 = first - (unsigned)row0 * nblk;
   }
@@ -240,7 +241,8 @@ __global__ __launch_bounds__(256) void restore8_kernel(long rows, long cols, con
 // ---- launches ----
 
 struct grid8 {
-  unsigned nblk, grid;
+  unsigned nblk;
+  dim3 grid;
   int u, tail;
 };
 // blocks, workgroups and blocks per lane group (engine_rows.c holds rows * blocks under 2^31): 4
@@ -252,7 +254,8 @@ grid8 grid_of(long rows, long cols, bool in_place) {
   // gated SiLU of bf16 52 us against 62)
   g.tail = tail_of(cols, true) != WHOLE || (in_place && cols % 8) ? PIECES : WHOLE;
   g.u = g.tail != PIECES && rows * g.nblk >= 4L * kGroups * 2048 ? 4 : 1;
-  g.grid = (unsigned)((rows * g.nblk + g.u * kGroups - 1) / (g.u * kGroups));
+  const long n = (rows * g.nblk + g.u * kGroups - 1) / (g.u * kGroups), x = 1L << kGridX;
+  g.grid = n < x ? dim3((unsigned)n) : dim3((unsigned)x, (unsigned)((n + x - 1) / x));
   return g;
 }
 
@@ -262,17 +265,16 @@ struct num {
 };
 // calls go with the kernel's U and TAIL
 template <class F>
-void shaped(const grid8 &g, F go) {
-  if (g.tail == PIECES) go(num<1>(), num<PIECES>());
-  else if (g.u == 4) go(num<4>(), num<WHOLE>());
-  else go(num<1>(), num<WHOLE>());
+int shaped(const grid8 &g, F go) {
+  if (g.tail == PIECES) return go(num<1>(), num<PIECES>());
+  if (g.u == 4) return go(num<4>(), num<WHOLE>());
+  return go(num<1>(), num<WHOLE>());
 }
 
 template <class T, int KIND, bool GATE>
 int act_go(const ext_mpi_amd_act &d, hipStream_t st) {
   const grid8 g = grid_of(d.rows, d.cols, d.h && (d.h == d.a || d.h == d.b));
-  shaped(g, [&](auto u, auto tail) { act_kernel<T, KIND, GATE, u.v, tail.v><<<g.grid, 256, 0, st>>>(d, g.nblk); });
-  return launched();
+  return shaped(g, [&](auto u, auto tail) { return launch(act_kernel<T, KIND, GATE, u.v, tail.v>, g.grid, 256, st, d, g.nblk); });
 }
 
 template <class T, int KIND>
@@ -294,8 +296,9 @@ int act_t(const ext_mpi_amd_act &d, hipStream_t st) {
 template <class T, int KIND, bool GATE>
 int act_grad_go(const ext_mpi_amd_act_grad &d, hipStream_t st) {
   const grid8 g = grid_of(d.rows, d.cols, d.da == d.dh || d.db == d.dh || d.h == d.dh);
-  shaped(g, [&](auto u, auto tail) { act_grad_kernel<T, KIND, GATE, u.v, tail.v><<<g.grid, 256, 0, st>>>(d, g.nblk); });
-  return launched();
+  return shaped(g, [&](auto u, auto tail) {
+    return launch(act_grad_kernel<T, KIND, GATE, u.v, tail.v>, g.grid, 256, st, d, g.nblk);
+  });
 }
 
 template <class T, int KIND>
@@ -317,10 +320,9 @@ template <class T>
 int restore_t(long rows, long cols, const signed char *q, long q_stride, const float *scale, void *x, long x_stride,
               hipStream_t st) {
   const grid8 g = grid_of(rows, cols, false);
-  shaped(g, [&](auto u, auto tail) {
-    restore8_kernel<T, u.v, tail.v><<<g.grid, 256, 0, st>>>(rows, cols, q, q_stride, scale, (T *)x, x_stride, g.nblk);
+  return shaped(g, [&](auto u, auto tail) {
+    return launch(restore8_kernel<T, u.v, tail.v>, g.grid, 256, st, rows, cols, q, q_stride, scale, (T *)x, x_stride, g.nblk);
   });
-  return launched();
 }
 
 } // namespace

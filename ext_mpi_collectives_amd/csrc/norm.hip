@@ -90,9 +90,8 @@ int emac_gpu_layernorm_grad(const ext_mpi_amd_layernorm_grad *d, float *part, vo
   }
   if (!sums) return 0;
   // no rows: the sums are zeros
-  colsum_kernel<<<dim3((unsigned)((d->cols + 31) / 32), 2), 1024, 0, st>>>(part, d->rows > 0 ? s.grid : 0, d->cols, d->dweight,
-                                                                         d->dbias, d->gdtype, d->accumulate);
-  return launched();
+  return launch(colsum_kernel, dim3((unsigned)((d->cols + 31) / 32), 2), 1024, st, part, d->rows > 0 ? s.grid : 0, d->cols,
+                d->dweight, d->dbias, d->gdtype, d->accumulate);
 }
 
 } // extern "C"

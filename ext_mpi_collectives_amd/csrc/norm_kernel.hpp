@@ -69,23 +69,29 @@ struct slot {
   __device__ void store(void *row, raw8<T> v) const {
     if (in()) store8<T, again>((T *)row, (unsigned)(TAIL == WHOLE ? c : own), v, TAIL == WHOLE ? 8 : n);
   }
-  // the sum of f's, and of f h's, own elements
+  // f's, and f h's, own elements added to s0 and s1, each vector's first among themselves: short chains
   __device__ void sums(f8 f, f8 h, float &s0, float &s1) const {
     int m = n;
     asm volatile("" : "+v"(m)); // or the branches of several vectors are threaded together, and their registers
+    float t0, t1;
     if (m >= 8) {
+      t0 = f[0];
+      t1 = f[0] * h[0];
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        s0 += f[j];
-        s1 += f[j] * h[j];
+      for (int j = 1; j < 8; j++) {
+        t0 += f[j];
+        t1 += f[j] * h[j];
       }
     } else {
+      t0 = t1 = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        s0 += mine(j) ? f[j] : 0.0f;
-        s1 += mine(j) ? f[j] * h[j] : 0.0f;
+        t0 += mine(j) ? f[j] : 0.0f;
+        t1 += mine(j) ? f[j] * h[j] : 0.0f;
       }
     }
+    s0 += t0;
+    s1 += t1;
   }
 };
 template <class T>
@@ -191,7 +197,7 @@ struct weights {
 
 template <class T, class W, int MODE, int NV, bool MULTI, int TAIL>
 __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void layernorm_kernel(const ext_mpi_amd_layernorm d) {
-  constexpr bool AHEAD = !MULTI && NV * sizeof(T) <= 8; // the next row's loads are issued before this row's sums
+  constexpr bool AHEAD = !MULTI && NV * sizeof(T) <= 12; // the next row's loads are issued before this row's sums
   const lanes<MODE> ln;
   const int l = ln.l, per = ln.per, cols = (int)d.cols;
   const int nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
@@ -536,7 +542,8 @@ inline row_shape row_shape_of(long cols) {
 // of them cost more than they hide, the gradient (not `most`) above all: each leaves a partial row.
 inline int per_cu(const row_shape &s, long cols, int dtype, bool most) {
   const long bytes = (s.mode < 512 ? 256 / s.mode : 1) * cols * (dtype == EXT_MPI_AMD_FLOAT ? 4 : 2);
-  const long by_bytes = (8192 + bytes / 2) / bytes, by_waves = most ? (512 + s.block - 1) / s.block : s.block > 256 ? 1 : 512 / s.block;
+  const long by_bytes = (8192 + bytes / 2) / bytes;
+  const long by_waves = most ? (512 + s.block - 1) / s.block : s.block > 256 ? 1 : 512 / s.block;
   const long cap = most ? 8 : 5;
   return (int)(by_bytes > cap ? cap : by_bytes > by_waves ? by_bytes : by_waves);
 }
@@ -547,8 +554,7 @@ int norm_go(const ext_mpi_amd_layernorm &d, const row_shape &s, hipStream_t st) 
   const long want = (d.rows + rows - 1) / rows;
   const long most = (long)EMAC_NORM_CUS * per_cu(s, d.cols, d.dtype, true);
   const int grid = (int)(want < most ? want : most);
-  layernorm_kernel<T, W, MODE, NV, MULTI, TAIL><<<grid, s.block, 0, st>>>(d);
-  return launched();
+  return launch(layernorm_kernel<T, W, MODE, NV, MULTI, TAIL>, grid, s.block, st, d);
 }
 
 template <class T, class W, int MODE, int NV>
@@ -614,9 +620,8 @@ inline grad_shape grad_shape_of(const ext_mpi_amd_layernorm_grad &d) {
 template <class T, class W, int MODE, int NV, int TAIL>
 int apart_go(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, hipStream_t st) {
   const auto go = [&](int rows, int tiles) {
-    if (d.q) layernorm_grad_apart_kernel<T, W, MODE, NV, true, TAIL><<<rows + tiles, s.r.block, 0, st>>>(d, rows);
-    else layernorm_grad_apart_kernel<T, W, MODE, NV, false, TAIL><<<rows + tiles, s.r.block, 0, st>>>(d, rows);
-    return launched();
+    if (d.q) return launch(layernorm_grad_apart_kernel<T, W, MODE, NV, true, TAIL>, rows + tiles, s.r.block, st, d, rows);
+    return launch(layernorm_grad_apart_kernel<T, W, MODE, NV, false, TAIL>, rows + tiles, s.r.block, st, d, rows);
   };
   if (!s.before || !s.tiles || !s.grid) return go(s.grid, s.tiles);
   const int rc = go(0, s.tiles);
@@ -625,9 +630,8 @@ int apart_go(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, hipStream
 
 template <class T, class W, int MODE, int NV, bool MULTI, int TAIL>
 int grad_go(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part, hipStream_t st) {
-  if (d.q) layernorm_grad_kernel<T, W, MODE, NV, true, MULTI, TAIL><<<s.grid, s.r.block, 0, st>>>(d, part);
-  else layernorm_grad_kernel<T, W, MODE, NV, false, MULTI, TAIL><<<s.grid, s.r.block, 0, st>>>(d, part);
-  return launched();
+  if (d.q) return launch(layernorm_grad_kernel<T, W, MODE, NV, true, MULTI, TAIL>, s.grid, s.r.block, st, d, part);
+  return launch(layernorm_grad_kernel<T, W, MODE, NV, false, MULTI, TAIL>, s.grid, s.r.block, st, d, part);
 }
 
 template <class T, class W, int MODE, int NV>
@@ -658,9 +662,8 @@ int grad_w(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part
 template <class T>
 int grad_cols(const ext_mpi_amd_layernorm_grad &d, int slices, float *part, hipStream_t st) {
   const dim3 grid(slices, (unsigned)((d.cols + 511) / 512));
-  if (d.q) layernorm_cols_kernel<T, true><<<grid, 256, 0, st>>>(d, part);
-  else layernorm_cols_kernel<T, false><<<grid, 256, 0, st>>>(d, part);
-  return launched();
+  if (d.q) return launch(layernorm_cols_kernel<T, true>, grid, 256, st, d, part);
+  return launch(layernorm_cols_kernel<T, false>, grid, 256, st, d, part);
 }
 
 // whether weights of their own type need their own kernels

@@ -348,8 +348,14 @@ __device__ inline f8 bytes(u2 q) {
 }
 __device__ inline f8 restore(u2 q, float scale) { return bytes(q) * scale; }
 
-// ---- launch helper: the grid must not be empty, and a launch error is the caller's ----
-inline int launched() { return hipGetLastError() == hipSuccess ? 0 : EMAC_ERR_DEVICE; }
+// A launch, with its own error and not one that an earlier call of the program left behind.
+template <class... A, class... V>
+int launch(void (*kernel)(A...), dim3 grid, int block, hipStream_t stream, V... values) {
+  return [&](A... a) {
+    void *args[] = {(void *)&a...};
+    return hipLaunchKernel((const void *)kernel, grid, dim3(block), args, 0, stream) == hipSuccess ? 0 : EMAC_ERR_DEVICE;
+  }(values...);
+}
 
 } // namespace emac_rows
 #endif

@@ -2,8 +2,9 @@
 checkpoint) in 32 bits, the rest in 64, and how far a 32-bit computation may be from that.
 
 U is half a step of a 32-bit float at 1. The bounds count roundings on the longest path of the
-computation: a row's sum adds at most 64 elements in a lane and 32 partial sums across lanes, so its
-error is at most 96 U times the sum of magnitudes; 128 U covers the few operations around it."""
+computation: a row's sum adds 8 elements of a vector, at most 16 vectors of a lane and 64 partial sums
+across lanes, so its error is under 96 U times the sum of magnitudes; 128 U covers the few operations
+around it."""
 import math
 
 import torch
@@ -85,7 +86,7 @@ def layernorm_grad(g, x, mean, rstd, w, dsum):
         dx = dx + dsum.double()
         ex = ex + 2 * U * (dx.abs() + dsum.double().abs())
     # a column's sum: rows / 16 terms in a lane at the most (16 rows side by side in one workgroup), then
-    # 15 of those, then up to 1024 / 8 partial rows and 8 of their sums
+    # 15 of those, then a 32nd of up to 1280 partial rows and 32 of their sums: 87, and 155 are counted
     depth = (-(-rows // 16) + 15 + 128 + 8 + 4) * U
     return dx, ex, (g * xh).sum(0), depth * (g * xh).abs().sum(0) + (g.abs() * exh).sum(0), g.sum(0), depth * g.abs().sum(0)
 

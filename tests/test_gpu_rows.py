@@ -160,6 +160,51 @@ def test_layernorm_grad_many_rows(rows, cols, t):
     assert torch.equal(dx, out[0][0]) and torch.equal(db, out[0][2])
 
 
+WIDTHS = [(70001, 5), (70000, 40), (33333, 72), (9001, 264), (3000, 1300), (1025, 4096), (700, 5000), (600, 5121), (550, 8192), (600, 10001),
+          (520, 12290), (510, 13000), (515, 16384), (300, 20001), (270, 33000)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("nsrc", [1, 3])
+@pytest.mark.parametrize("rows,cols", WIDTHS)
+def test_forward_and_gradient_over_many_rows(rows, cols, nsrc, t):
+    """Every width's kernels with more rows than workgroups: the norm with a checkpoint, then its gradient
+    from x and from the checkpoint, the checkpoint's with the norm's output again."""
+    dt, gen = ref.TYPES[t], rnd(rows + nsrc)
+    src = [torch.randn(rows, cols, device="cuda", generator=gen).to(dt) for _ in range(nsrc)]
+    w, b = (torch.randn(cols, device="cuda", generator=gen).to(dt) for _ in range(2))
+    x, y, y2, dx, dx8 = (torch.empty_like(src[0]) for _ in range(5))
+    mean, rstd = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    q, scale = torch.empty(rows, cols, dtype=torch.int8, device="cuda"), torch.empty(rows, -(-cols // 128), device="cuda")
+    dw, db, dw8, db8 = (torch.empty(cols, device="cuda") for _ in range(4))
+    go(emac.layernorm_init(rows, cols, CODE[dt], [v.data_ptr() for v in src], y.data_ptr(), weight=w.data_ptr(), bias=b.data_ptr(), sum=x.data_ptr(),
+                           mean=mean.data_ptr(), rstd=rstd.data_ptr(), q=q.data_ptr(), scale=scale.data_ptr()))
+    assert torch.equal(x, ref.fold(src))
+    rq, rscale = ref.save8(x)
+    assert torch.equal(q, rq) and torch.equal(scale, rscale)
+    _, rrstd, ry, by = ref.layernorm(x, w, b, 1e-5)
+    ref.close(y, ry, by)
+    ref.close(rstd, rrstd, rrstd * ref.stats_bounds(x, rrstd)[1])
+    kw = dict(weight=w.data_ptr(), gdtype=emac.FLOAT)
+    dys = [v.data_ptr() for v in src]  # any rows do as gradients
+    go(emac.layernorm_grad_init(rows, cols, CODE[dt], dys, mean.data_ptr(), rstd.data_ptr(), x=x.data_ptr(), dx=dx.data_ptr(), dweight=dw.data_ptr(),
+                                dbias=db.data_ptr(), **kw),
+       emac.layernorm_grad_init(rows, cols, CODE[dt], dys, mean.data_ptr(), rstd.data_ptr(), q=q.data_ptr(), scale=scale.data_ptr(), dx=dx8.data_ptr(),
+                                dweight=dw8.data_ptr(), dbias=db8.data_ptr(), dsum=x.data_ptr(), bias=b.data_ptr(), y=y2.data_ptr(), **kw))
+    g = src[0].float()
+    for v in src[1:]:
+        g = g + v.float()
+    xq = ref.restore8(rq, rscale)
+    for xv, o, ow, ob, ds in ((x, dx, dw, db, None), (xq, dx8, dw8, db8, x)):
+        rdx, bdx, rdw, bdw, rdb, bdb = ref.layernorm_grad(g, xv, mean, rstd, w, ds)
+        ref.close(o, rdx, bdx)
+        ref.close(ow, rdw, bdw)
+        ref.close(ob, rdb, bdb)
+    xh = (xq.double() - mean.double()[:, None]) * rstd.double()[:, None]
+    exh = 8 * ref.U * (xh.abs() + rstd.double()[:, None] * (xq.double().abs() + mean.double().abs()[:, None]))
+    ref.close(y2, xh * w.double() + b.double(), exh * w.double().abs() + 8 * ref.U * b.double().abs())
+
+
 @pytest.mark.parametrize("cols,t", [(200, "f32"), (1000, "f32"), (5000, "f32")])
 def test_layernorm_grad_by_differences(cols, t):
     """The change of L = sum(y r) along a direction of x, w and b, by central differences of the forward
@@ -430,6 +475,17 @@ def test_offsets_past_32_bits(t):
     ref.close(dw, rdw, bdw)
     go(emac.restore8_init(rows, cols, CODE[dt], q.data_ptr(), scale.data_ptr(), x.data_ptr(), q_stride=1 << 31, x_stride=ld))
     assert torch.equal(x, ref.restore8(rq, rscale).to(dt))
+
+
+def test_more_blocks_than_one_grid_dimension():
+    """2^28 and a few blocks, of one column each: 127 or -127, and back to the value's own bits."""
+    rows = (1 << 28) + 37
+    x = torch.randn(rows, 1, dtype=torch.bfloat16, device="cuda", generator=rnd(8))
+    x[x == 0] = 1
+    q, scale, back = torch.empty(rows, 1, dtype=torch.int8, device="cuda"), torch.empty(rows, 1, device="cuda"), torch.empty_like(x)
+    go(emac.save8_init(rows, 1, emac.BF16, x.data_ptr(), q.data_ptr(), scale.data_ptr()),
+       emac.restore8_init(rows, 1, emac.BF16, q.data_ptr(), scale.data_ptr(), back.data_ptr()))
+    assert torch.equal(q, (x.sign() * 127).to(torch.int8)) and torch.equal(back, x)
 
 
 def test_one_training_step_as_used():
