@@ -557,11 +557,27 @@ int norm_go(const ext_mpi_amd_layernorm &d, const row_shape &s, hipStream_t st) 
   return launch(layernorm_kernel<T, W, MODE, NV, MULTI, TAIL>, grid, s.block, st, d);
 }
 
+// Rows of 16 to 32 KB from one leaf: a workgroup of up to 16 waves with 32 bytes of the row to a lane,
+// where row_shape_of gives fewer waves more of it (float, 8192 x 5120 with residual, sum and checkpoint
+// 131 us against 168, 4096 x 8192 112 against 129; bf16 without 4096 x 10240 36.7 against 40.2).
+// Shorter rows are slower with more waves (bf16 4096 x 8192 38.3 against 25.1), and longer ones do not
+// fit the registers (float 4096 x 12288 90 against 79).
+template <class T, int NV>
+constexpr bool sixteen() {
+  return sizeof(T) == 4 ? NV == 2 : NV == 3 || NV == 4;
+}
+inline int sixteen_block(long cols, int esize) { return (int)((cols * esize + 31) / 32 + 63) / 64 * 64; }
+
 template <class T, class W, int MODE, int NV>
 int norm_nv(const ext_mpi_amd_layernorm &d, const row_shape &s, hipStream_t st) {
   if (tail_of(d.cols, d.q) == SHIFT) return norm_go<T, W, MODE, NV, true, SHIFT>(d, s, st);
   if (d.nsrc > 1) return norm_go<T, W, MODE, NV, true, WHOLE>(d, s, st);
-  return norm_go<T, W, MODE, NV, false, WHOLE>(d, s, st);
+  if constexpr (sixteen<T, NV>()) {
+    const int block = sixteen_block(d.cols, sizeof(T));
+    return norm_go<T, W, 1024, 4 / sizeof(T), false, WHOLE>(d, row_shape{1024, 4 / (int)sizeof(T), block}, st);
+  } else {
+    return norm_go<T, W, MODE, NV, false, WHOLE>(d, s, st);
+  }
 }
 
 template <class T, class W>
@@ -640,7 +656,15 @@ int grad_nv(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *par
     return s.apart ? apart_go<T, W, MODE, NV, SHIFT>(d, s, st) : grad_go<T, W, MODE, NV, true, SHIFT>(d, s, part, st);
   if (s.apart) return apart_go<T, W, MODE, NV, WHOLE>(d, s, st);
   if (d.nsrc > 1 || d.y) return grad_go<T, W, MODE, NV, true, WHOLE>(d, s, part, st);
-  return grad_go<T, W, MODE, NV, false, WHOLE>(d, s, part, st);
+  if constexpr (sizeof(T) == 4 && NV == 2) {
+    // as in sixteen (float 8192 x 5120 127 us against 131); 16-bit types' two vectors and their column
+    // sums would not fit the registers
+    grad_shape z = s;
+    z.r = row_shape{1024, 1, sixteen_block(d.cols, 4)};
+    return grad_go<T, W, 1024, 1, false, WHOLE>(d, z, part, st);
+  } else {
+    return grad_go<T, W, MODE, NV, false, WHOLE>(d, s, part, st);
+  }
 }
 
 template <class T, class W>
