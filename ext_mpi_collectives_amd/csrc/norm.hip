@@ -60,8 +60,8 @@ int emac_gpu_layernorm(const ext_mpi_amd_layernorm *d, void *stream) {
 
 size_t emac_gpu_layernorm_grad_ws(const ext_mpi_amd_layernorm_grad *d) {
   const grad_shape s = grad_shape_of(*d);
-  if (s.apart || s.grid <= 1 || !(d->dweight || d->dbias)) return 0;
-  return sizeof(float) * 2 * (size_t)d->cols * (size_t)s.grid;
+  if (s.apart || s.parts <= 1 || !(d->dweight || d->dbias)) return 0;
+  return sizeof(float) * 2 * (size_t)d->cols * (size_t)s.parts;
 }
 
 int emac_gpu_layernorm_grad(const ext_mpi_amd_layernorm_grad *d, float *part, void *stream) {
@@ -72,9 +72,9 @@ int emac_gpu_layernorm_grad(const ext_mpi_amd_layernorm_grad *d, float *part, vo
   if (d->rows > 0) {
     if (s.wide && sums && !s.apart) { // the column sums first: dx may overwrite what they read
       switch (d->dtype) {
-      case EXT_MPI_AMD_FLOAT: rc = grad_cols<float>(*d, s.grid, part, st); break;
-      case EXT_MPI_AMD_BF16: rc = grad_cols<bf16>(*d, s.grid, part, st); break;
-      case EXT_MPI_AMD_HALF: rc = grad_cols<half>(*d, s.grid, part, st); break;
+      case EXT_MPI_AMD_FLOAT: rc = grad_cols<float>(*d, s.parts, part, st); break;
+      case EXT_MPI_AMD_BF16: rc = grad_cols<bf16>(*d, s.parts, part, st); break;
+      case EXT_MPI_AMD_HALF: rc = grad_cols<half>(*d, s.parts, part, st); break;
       }
       if (rc) return rc;
     }
@@ -90,7 +90,7 @@ int emac_gpu_layernorm_grad(const ext_mpi_amd_layernorm_grad *d, float *part, vo
   }
   if (!sums) return 0;
   // no rows: the sums are zeros
-  return launch(colsum_kernel, dim3((unsigned)((d->cols + 31) / 32), 2), 1024, st, part, d->rows > 0 ? s.grid : 0, d->cols,
+  return launch(colsum_kernel, dim3((unsigned)((d->cols + 31) / 32), 2), 1024, st, part, d->rows > 0 ? s.parts : 0, d->cols,
                 d->dweight, d->dbias, d->gdtype, d->accumulate);
 }
 

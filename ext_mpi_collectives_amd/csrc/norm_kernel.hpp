@@ -41,6 +41,7 @@ struct lanes {
 // them out of every sum and store.
 template <int TAIL>
 struct slot {
+  static constexpr int kTail = TAIL;
   int own, c, n; // first column of its own, of those it loads; its own elements (0 or less: none)
   __device__ slot(int i, int per, int l, int cols, bool live) {
     own = (l + i * per) * 8;
@@ -198,6 +199,7 @@ struct weights {
 template <class T, class W, int MODE, int NV, bool MULTI, int TAIL>
 __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void layernorm_kernel(const ext_mpi_amd_layernorm d) {
   constexpr bool AHEAD = !MULTI && NV * sizeof(T) <= 12; // the next row's loads are issued before this row's sums
+  constexpr bool EACH = MULTI && MODE == 1024 && NV > 1; // wide rows, folded vector by vector: x alone stays in registers
   const lanes<MODE> ln;
   const int l = ln.l, per = ln.per, cols = (int)d.cols;
   const int nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
@@ -224,15 +226,21 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
     const bool live = ln.kOneRow || row < d.rows;
     raw8<T> x[NV];
     float s[1] = {0.0f};
-    if (!AHEAD) load(within(row));
-    f8 sum[MULTI ? NV : 1];
-    if constexpr (MULTI) fold_rows<T, NV, TAIL>(sum, d.src, d.nsrc, within(row), d.src_stride, per, l, cols);
+    if (!AHEAD && !EACH) load(within(row));
+    f8 sum[MULTI && !EACH ? NV : 1];
+    if constexpr (MULTI && !EACH) fold_rows<T, NV, TAIL>(sum, d.src, d.nsrc, within(row), d.src_stride, per, l, cols);
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       const slot<TAIL> at(i, per, l, cols, true);
+      if constexpr (EACH) {
+        if (d.residual) nr[i] = at.template load<T>(row_of<T>(d.residual, row, d.residual_stride));
+        f8 one[1];
+        fold_rows<T, 1, TAIL>(one, d.src, d.nsrc, row, d.src_stride, per, l + i * per, cols);
+        sum[0] = one[0];
+      }
       if (MULTI || d.residual) {
         f8 f;
-        if (MULTI) f = sum[MULTI ? i : 0];
+        if (MULTI) f = sum[MULTI && !EACH ? i : 0];
         else f = widen<T>(nx[MULTI ? 0 : i]);
         if (d.residual) f += widen<T>(nr[i]);
         x[i] = round_to<T>(f);
@@ -520,6 +528,58 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
   else cols_tile<T, 8, Q8, true, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr);
 }
 
+// Rows of more than 16384 columns. Held in registers they spill: a workgroup reads its row twice, for
+// the sums and for dx, the second time from the caches. The workgroups behind `blocks` as above.
+template <class T, class W, bool Q8>
+__global__ __launch_bounds__(512) void layernorm_grad_wide_kernel(const ext_mpi_amd_layernorm_grad d, int blocks) {
+  if ((int)blockIdx.x >= blocks) return cols_tile<T, 8, Q8, true, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr);
+  const int cols = (int)d.cols, full = cols / 8, nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
+  const float inv = 1.0f / (float)cols;
+  __shared__ float red[2][lanes<512>::kSlots][2];
+  row_sum<512, 2> sum_row(red);
+  for (long row = blockIdx.x; row < d.rows; row += blocks) {
+    const float rstd = d.rstd[row], shift = -d.mean[row] * rstd;
+    float s[2] = {0.0f, 0.0f}, c1, c2;
+    // vector v of the row: into the sums (and y), or into dx. Each lane loads its own elements alone,
+    // which dx may replace.
+    const auto take = [&](auto at, bool sums, int v) {
+      typedef decltype(at) slot_t;
+      row8<T, Q8, slot_t::kTail> x;
+      x.load(d, row, at, nblk);
+      raw8<T> more;
+      if (!sums && d.dsum) more = at.template load<T>(row_of<T>(d.dsum, row, d.dsum_stride));
+      f8 g[1], ww = 1.0f;
+      if (d.weight) ww = widen<W>(at.template load<W, true>(d.weight));
+      fold_rows<T, 1, slot_t::kTail>(g, d.dy, d.nsrc, row, d.dy_stride, 0, v, cols);
+      const f8 xh = x.normed(rstd, shift, at);
+      if (sums) {
+        if (d.y) {
+          f8 y = xh * ww;
+          if (d.bias) y += widen<W>(at.template load<W, true>(d.bias));
+          at.template store<T>((T *)d.y + row * d.y_stride, round_to<T>(y));
+        }
+        at.sums(g[0] * ww, xh, s[0], s[1]);
+      } else {
+        f8 dx = xh * c2 + c1;
+        dx += g[0] * ww * rstd;
+        if (d.dsum) dx += widen<T>(more);
+        at.template store<T>((T *)d.dx + row * d.dx_stride, round_to<T>(dx));
+      }
+    };
+    const auto pass = [&](bool sums) {
+#pragma unroll 2
+      for (int v = threadIdx.x; v < full; v += 512) take(slot<WHOLE>(0, 0, v, cols, true), sums, v);
+      if (cols % 8 && (int)threadIdx.x == full % 512) take(slot<PIECES>(0, 0, full, cols, true), sums, full);
+    };
+    if (d.dx || d.y) pass(true);
+    if (!d.dx) continue;
+    sum_row(s);
+    c1 = -s[0] * inv * rstd;
+    c2 = -s[1] * inv * rstd;
+    pass(false);
+  }
+}
+
 // ---- launches ----
 
 #define EMAC_NORM_CUS 256 // compute units of the part
@@ -531,8 +591,8 @@ struct row_shape {
 inline row_shape row_shape_of(long cols) {
   const long v = (cols + 7) / 8; // vectors in a row
   row_shape s;
-  s.mode = v <= 16 ? 16 : v <= 64 ? 64 : 512;
-  s.nv = v <= 512 ? 1 : v <= 1024 ? 2 : v <= 1536 ? 3 : v <= 2048 ? 4 : v <= 4096 ? 8 : 16;
+  s.mode = v <= 16 ? 16 : v <= 64 ? 64 : v <= 2048 ? 512 : 1024;
+  s.nv = v <= 512 ? 1 : v <= 1024 ? 2 : v <= 1536 ? 3 : v <= 4096 ? 4 : 8;
   s.block = s.mode < 512 ? 256 : (int)((v + s.nv - 1) / s.nv + 63) / 64 * 64;
   return s;
 }
@@ -596,25 +656,26 @@ int norm_w(const ext_mpi_amd_layernorm &d, hipStream_t st) {
   if (s.nv == 1) return norm_nv<T, W, 512, 1>(d, s, st);
   if (s.nv == 2) return norm_nv<T, W, 512, 2>(d, s, st);
   if (s.nv == 3) return norm_nv<T, W, 512, 3>(d, s, st);
-  if (s.nv == 4) return norm_nv<T, W, 512, 4>(d, s, st);
+  if (s.mode == 512) return norm_nv<T, W, 512, 4>(d, s, st);
   // wider: the forms that take any number of leaves
-  if (s.nv == 8) return tail == WHOLE ? norm_go<T, W, 512, 8, true, WHOLE>(d, s, st) : norm_go<T, W, 512, 8, true, SHIFT>(d, s, st);
-  return tail == WHOLE ? norm_go<T, W, 512, 16, true, WHOLE>(d, s, st) : norm_go<T, W, 512, 16, true, SHIFT>(d, s, st);
+  if (s.nv == 4) return tail == WHOLE ? norm_go<T, W, 1024, 4, true, WHOLE>(d, s, st) : norm_go<T, W, 1024, 4, true, SHIFT>(d, s, st);
+  return tail == WHOLE ? norm_go<T, W, 1024, 8, true, WHOLE>(d, s, st) : norm_go<T, W, 1024, 8, true, SHIFT>(d, s, st);
 }
 
-// the gradient's launch: `grid` workgroups take the rows, and each leaves a partial row of column
-// sums; or (apart) `tiles` more take the column sums, in a launch before the rows' where dx replaces
+// the gradient's launch: `grid` workgroups take the rows, and each (of wide rows: each slice of the rows
+// in a launch of its own) leaves a partial row of column sums; or (apart) `tiles` more take the column sums, in a launch before the rows' where dx replaces
 // what they read (the same sums either way)
 struct grad_shape {
   row_shape r;
-  int grid, tiles;
+  int grid, tiles, parts; // parts: partial rows
   bool apart, before;
   bool wide; // two column sums beside a row's values no longer fit in registers
 };
 inline grad_shape grad_shape_of(const ext_mpi_amd_layernorm_grad &d) {
   grad_shape s;
   s.r = row_shape_of(d.cols);
-  s.wide = s.r.nv > 4;
+  s.wide = s.r.mode == 1024;
+  if (s.wide) s.r.block = 512;
   const bool sums = d.dweight || d.dbias;
   const long rows = s.r.mode < 512 ? 256 / s.r.mode : 1, want = (d.rows + rows - 1) / rows;
   // few rows: the second launch, which adds the partial rows, costs more than reading the rows twice,
@@ -627,21 +688,28 @@ inline grad_shape grad_shape_of(const ext_mpi_amd_layernorm_grad &d) {
   s.apart = sums && d.rows <= 4 * (lanes / 8) && twice <= 16L << 20;
   s.tiles = s.apart ? (int)((d.cols + 63) / 64) : 0;
   if (s.apart) s.r.block = lanes;
-  const long most = s.apart ? 2048 : (long)EMAC_NORM_CUS * per_cu(s.r, d.cols, d.dtype, false);
+  const long most = s.apart ? 2048 : (long)EMAC_NORM_CUS * (s.wide ? 2 : per_cu(s.r, d.cols, d.dtype, false));
   s.grid = (int)(want < most ? want : most);
+  s.parts = s.grid;
+  if (s.wide) { // 8 workgroups to a CU for the column sums
+    const int slices = 2048 / (int)((d.cols + 511) / 512);
+    s.parts = s.parts < slices ? s.parts : slices;
+  }
   if (s.apart && !d.dx && !d.y) s.grid = 0;
   return s;
 }
 
+typedef void apart_kernel(const ext_mpi_amd_layernorm_grad, int);
+inline int apart_go(apart_kernel *k, const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, hipStream_t st) {
+  if (!s.before || !s.tiles || !s.grid) return launch(k, s.grid + s.tiles, s.r.block, st, d, s.grid);
+  const int rc = launch(k, s.tiles, s.r.block, st, d, 0);
+  return rc ? rc : launch(k, s.grid, s.r.block, st, d, s.grid);
+}
+
 template <class T, class W, int MODE, int NV, int TAIL>
-int apart_go(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, hipStream_t st) {
-  const auto go = [&](int rows, int tiles) {
-    if (d.q) return launch(layernorm_grad_apart_kernel<T, W, MODE, NV, true, TAIL>, rows + tiles, s.r.block, st, d, rows);
-    return launch(layernorm_grad_apart_kernel<T, W, MODE, NV, false, TAIL>, rows + tiles, s.r.block, st, d, rows);
-  };
-  if (!s.before || !s.tiles || !s.grid) return go(s.grid, s.tiles);
-  const int rc = go(0, s.tiles);
-  return rc ? rc : go(s.grid, 0);
+int apart_t(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, hipStream_t st) {
+  if (d.q) return apart_go(layernorm_grad_apart_kernel<T, W, MODE, NV, true, TAIL>, d, s, st);
+  return apart_go(layernorm_grad_apart_kernel<T, W, MODE, NV, false, TAIL>, d, s, st);
 }
 
 template <class T, class W, int MODE, int NV, bool MULTI, int TAIL>
@@ -653,8 +721,8 @@ int grad_go(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *par
 template <class T, class W, int MODE, int NV>
 int grad_nv(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part, hipStream_t st) {
   if (tail_of(d.cols, d.q) == SHIFT)
-    return s.apart ? apart_go<T, W, MODE, NV, SHIFT>(d, s, st) : grad_go<T, W, MODE, NV, true, SHIFT>(d, s, part, st);
-  if (s.apart) return apart_go<T, W, MODE, NV, WHOLE>(d, s, st);
+    return s.apart ? apart_t<T, W, MODE, NV, SHIFT>(d, s, st) : grad_go<T, W, MODE, NV, true, SHIFT>(d, s, part, st);
+  if (s.apart) return apart_t<T, W, MODE, NV, WHOLE>(d, s, st);
   if (d.nsrc > 1 || d.y) return grad_go<T, W, MODE, NV, true, WHOLE>(d, s, part, st);
   if constexpr (sizeof(T) == 4 && NV == 2) {
     // as in sixteen (float 8192 x 5120 127 us against 131); 16-bit types' two vectors and their column
@@ -671,16 +739,17 @@ template <class T, class W>
 int grad_w(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part, hipStream_t st) {
   const int tail = tail_of(d.cols, d.q);
   if (tail == PIECES)
-    return s.apart ? apart_go<T, W, 16, 1, PIECES>(d, s, st) : grad_go<T, W, 16, 1, true, PIECES>(d, s, part, st);
+    return s.apart ? apart_t<T, W, 16, 1, PIECES>(d, s, st) : grad_go<T, W, 16, 1, true, PIECES>(d, s, part, st);
+  if (s.wide) { // the column sums, if not apart, have a launch of their own before this one
+    if (d.q) return apart_go(layernorm_grad_wide_kernel<T, W, true>, d, s, st);
+    return apart_go(layernorm_grad_wide_kernel<T, W, false>, d, s, st);
+  }
   if (s.r.mode == 16) return grad_nv<T, W, 16, 1>(d, s, part, st);
   if (s.r.mode == 64) return grad_nv<T, W, 64, 1>(d, s, part, st);
   if (s.r.nv == 1) return grad_nv<T, W, 512, 1>(d, s, part, st);
   if (s.r.nv == 2) return grad_nv<T, W, 512, 2>(d, s, part, st);
   if (s.r.nv == 3) return grad_nv<T, W, 512, 3>(d, s, part, st);
   if (s.r.nv == 4) return grad_nv<T, W, 512, 4>(d, s, part, st);
-  // wide: the rows alone (the column sums, if any, have a launch of their own before this one)
-  if (s.r.nv == 8) return tail == WHOLE ? apart_go<T, W, 512, 8, WHOLE>(d, s, st) : apart_go<T, W, 512, 8, SHIFT>(d, s, st);
-  return tail == WHOLE ? apart_go<T, W, 512, 16, WHOLE>(d, s, st) : apart_go<T, W, 512, 16, SHIFT>(d, s, st);
 }
 
 template <class T>
