@@ -248,6 +248,11 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
         x[i] = nx[MULTI ? 0 : i];
       }
       x[i] = at.template put<T>(x[i]);
+      if (EACH && NV > 4 && i % 2) { // two vectors' loads in flight: all of them would spill
+        hold(x[i - (NV > 4)]);
+        hold(x[i]);
+        asm volatile("" ::: "memory");
+      }
     }
     if (AHEAD) load(within(row + step));
 #pragma unroll
@@ -262,6 +267,7 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
 #pragma unroll
       for (int i = 0; i < NV; i++) {
         const slot<TAIL> at(i, per, l, cols, true);
+        if (EACH) hold(x[i]); // or its floats, and then the differences, stay in registers beside x
         const f8 f = widen<T>(x[i]) - mean;
         float none = 0.0f;
         at.sums(f * f, (f8)0.0f, s[0], none);
@@ -276,6 +282,7 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
       for (int i = 0; i < NV; i++) {
         const slot<TAIL> at(i, per, l, cols, live);
         if (!d.y) continue;
+        if (EACH) hold(x[i]);
         const f8 f = (widen<T>(x[i]) - mean) * rstd * w.at(i, at) + b.at(i, at);
         at.template store<T>((T *)d.y + row * d.y_stride, round_to<T>(f));
       }
