@@ -481,7 +481,7 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
 template <class T, int LANES, bool Q8, bool MULTI, int TAIL>
 __device__ inline void cols_tile(const ext_mpi_amd_layernorm_grad &d, int tile, int slice, int slices, float *part) {
   constexpr int C = 8 * LANES;
-  __shared__ float comb[2][512 / LANES][C];
+  __shared__ float comb[2][512 / LANES][C]; // of up to 512 lanes
   const int l = threadIdx.x % LANES, k0 = threadIdx.x / LANES, R = blockDim.x / LANES;
   const int cols = (int)d.cols, nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
   const slot<TAIL> at(0, 0, tile * LANES + l, cols, true);
@@ -525,21 +525,22 @@ __global__ __launch_bounds__(256) void layernorm_cols_kernel(const ext_mpi_amd_l
 }
 
 // Rows without column sums, and in the workgroups behind theirs (from `blocks` on) the column sums of
-// 64 columns each over all rows: the rows are read twice, but nothing waits for anything.
+// 32 columns each over all rows: the rows are read twice, but nothing waits for anything. Fewer columns
+// to a workgroup, more rows at a time (256 x 2048 bf16 6.9 us against 8.6 with 64 columns).
 template <class T, class W, int MODE, int NV, bool Q8, int TAIL>
 __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void layernorm_grad_apart_kernel(
     const ext_mpi_amd_layernorm_grad d, int blocks) {
   if ((int)blockIdx.x < blocks) grad_rows<T, W, MODE, NV, Q8, true, TAIL, false>(d, blockIdx.x, blocks, nullptr);
-  else if (TAIL == PIECES) cols_tile<T, 8, Q8, true, PIECES>(d, blockIdx.x - blocks, 0, 1, nullptr);
-  else if (d.nsrc == 1) cols_tile<T, 8, Q8, false, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr);
-  else cols_tile<T, 8, Q8, true, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr);
+  else if (TAIL == PIECES) cols_tile<T, 4, Q8, true, PIECES>(d, blockIdx.x - blocks, 0, 1, nullptr);
+  else if (d.nsrc == 1) cols_tile<T, 4, Q8, false, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr);
+  else cols_tile<T, 4, Q8, true, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr);
 }
 
 // Rows of more than 16384 columns. Held in registers they spill: a workgroup reads its row twice, for
 // the sums and for dx, the second time from the caches. The workgroups behind `blocks` as above.
 template <class T, class W, bool Q8>
 __global__ __launch_bounds__(512) void layernorm_grad_wide_kernel(const ext_mpi_amd_layernorm_grad d, int blocks) {
-  if ((int)blockIdx.x >= blocks) return cols_tile<T, 8, Q8, true, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr);
+  if ((int)blockIdx.x >= blocks) return cols_tile<T, 4, Q8, true, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr);
   const int cols = (int)d.cols, full = cols / 8, nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
   const float inv = 1.0f / (float)cols;
   __shared__ float red[2][lanes<512>::kSlots][2];
@@ -669,9 +670,9 @@ int norm_w(const ext_mpi_amd_layernorm &d, hipStream_t st) {
   return tail == WHOLE ? norm_go<T, W, 1024, 8, true, WHOLE>(d, s, st) : norm_go<T, W, 1024, 8, true, SHIFT>(d, s, st);
 }
 
-// the gradient's launch: `grid` workgroups take the rows, and each (of wide rows: each slice of the rows
-// in a launch of its own) leaves a partial row of column sums; or (apart) `tiles` more take the column sums, in a launch before the rows' where dx replaces
-// what they read (the same sums either way)
+// the gradient's launch: `grid` workgroups take the rows, and each leaves a partial row of column sums
+// (of wide rows: each slice of the rows does, in a launch of its own); or (apart) `tiles` more take the
+// column sums, in a launch before the rows' where dx replaces what they read (the same sums either way)
 struct grad_shape {
   row_shape r;
   int grid, tiles, parts; // parts: partial rows
@@ -685,15 +686,16 @@ inline grad_shape grad_shape_of(const ext_mpi_amd_layernorm_grad &d) {
   if (s.wide) s.r.block = 512;
   const bool sums = d.dweight || d.dbias;
   const long rows = s.r.mode < 512 ? 256 / s.r.mode : 1, want = (d.rows + rows - 1) / rows;
-  // few rows: the second launch, which adds the partial rows, costs more than reading the rows twice,
-  // up to 4 of them to a lane (bf16, 4096 columns: 32 rows 4.5 us against 6.3, 256 rows 7.0 against
-  // 10.7, 512 rows, 8 to a lane, 12.0 against 11.1)
+  // few rows: the second launch, which adds the partial rows, costs more than reading the rows twice
+  // (bf16, one leaf: 32 x 4096 4.5 us against 6.3, 200 x 1024 5.9 against 7.5, 256 x 2048 6.9 against
+  // 8.9, but 512 x 4096 13.8 against 11.5; float, 4 leaves: 64 x 1024 5.0 against 6.5, but 200 x 1024
+  // 10.2 against 7.1)
   s.before = d.dx && d.dx == d.x;
   for (int i = 0; i < d.nsrc; i++) s.before = s.before || (d.dx && d.dx == d.dy[i]);
   const long twice = d.rows * d.cols * (d.nsrc + 1) * (d.dtype == EXT_MPI_AMD_FLOAT ? 4 : 2);
   const int lanes = s.r.block < 256 ? 256 : s.r.block; // more rows at a time for the column sums
-  s.apart = sums && d.rows <= 4 * (lanes / 8) && twice <= 16L << 20;
-  s.tiles = s.apart ? (int)((d.cols + 63) / 64) : 0;
+  s.apart = sums && d.rows <= (d.nsrc > 1 && lanes == 256 ? 128 : 256) && twice <= 16L << 20;
+  s.tiles = s.apart ? (int)((d.cols + 31) / 32) : 0;
   if (s.apart) s.r.block = lanes;
   const long most = s.apart ? 2048 : (long)EMAC_NORM_CUS * (s.wide ? 2 : per_cu(s.r, d.cols, d.dtype, false));
   s.grid = (int)(want < most ? want : most);
