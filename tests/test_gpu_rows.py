@@ -161,7 +161,7 @@ def test_layernorm_grad_many_rows(rows, cols, t):
 
 
 WIDTHS = [(70001, 5), (70000, 40), (33333, 72), (9001, 264), (3000, 1300), (1025, 4096), (700, 5000), (600, 5121), (550, 8192), (600, 10001),
-          (520, 12290), (510, 13000), (515, 16384), (300, 20001), (270, 33000)]
+          (520, 12290), (510, 13000), (515, 16384), (260, 16387), (300, 20001), (257, 32773), (270, 33000), (5, 65529)]
 
 
 @pytest.mark.parametrize("t", TYPES)
