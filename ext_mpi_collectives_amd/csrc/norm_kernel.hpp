@@ -622,7 +622,16 @@ template <class T, class W, int MODE, int NV, bool MULTI, int TAIL>
 int norm_go(const ext_mpi_amd_layernorm &d, const row_shape &s, hipStream_t st) {
   constexpr int rows = lanes<MODE>::kRows;
   const long want = (d.rows + rows - 1) / rows;
-  const long most = (long)EMAC_NORM_CUS * per_cu(s, d.cols, d.dtype, true);
+  long wgs = per_cu(s, d.cols, d.dtype, true);
+  if (MULTI && MODE == 512) {
+    // nothing is loaded ahead: 32 KB of leaves in flight to a CU, and with one vector to a lane two
+    // workgroups, as far as 16 waves go (bf16, 2 leaves: 16384 x 1024 26.2 us against 34.2 by the rule of
+    // the one-leaf kernels, 8192 x 4096 49.7 against 69.5; float 8192 x 4096 112 against 125)
+    const long bytes = d.nsrc * d.cols * (long)sizeof(T), fit = 1024 / s.block, least = NV == 1 ? 2 : 1;
+    const long fill = (32768 + bytes - 1) / bytes > least ? (32768 + bytes - 1) / bytes : least;
+    wgs = wgs > fill ? wgs : fill > fit ? fit : fill;
+  }
+  const long most = EMAC_NORM_CUS * wgs;
   const int grid = (int)(want < most ? want : most);
   return launch(layernorm_kernel<T, W, MODE, NV, MULTI, TAIL>, grid, s.block, st, d);
 }
