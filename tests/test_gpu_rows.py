@@ -637,6 +637,29 @@ def refused(code, f, *a, **kw):
     assert e.value.code == code, (e.value.code, code)
 
 
+def test_an_earlier_error_of_the_program_is_not_a_starts():
+    x = torch.randn(4, 256, device="cuda", generator=rnd(3))
+    y, q, scale, dw = torch.empty_like(x), torch.empty(4, 256, dtype=torch.int8, device="cuda"), torch.empty(4, 2, device="cuda"), torch.empty(256, device="cuda")
+    mean, rstd = torch.empty(4, device="cuda"), torch.empty(4, device="cuda")
+    hs = [emac.layernorm_init(4, 256, emac.FLOAT, [x.data_ptr()], y.data_ptr(), mean=mean.data_ptr(), rstd=rstd.data_ptr()),
+          emac.layernorm_grad_init(4, 256, emac.FLOAT, [x.data_ptr()], mean.data_ptr(), rstd.data_ptr(), x=x.data_ptr(), dweight=dw.data_ptr()),
+          emac.save8_init(4, 256, emac.FLOAT, x.data_ptr(), q.data_ptr(), scale.data_ptr()),
+          emac.act_init(4, 256, emac.FLOAT, emac.SILU, x.data_ptr(), y.data_ptr())]
+    stream = torch.cuda.current_stream().cuda_stream
+    for h in hs:
+        emac.set_stream(h, stream)
+    assert emac.lib().hipSetDevice(9999) != 0  # refused, and remembered by the runtime
+    try:
+        for h in hs:
+            emac.start(h)
+    finally:
+        emac.lib().hipGetLastError()
+    for h in hs:
+        emac.wait(h)
+        emac.done(h)
+    assert torch.equal(q, ref.save8(x)[0])
+
+
 def test_refusals_of_memory():
     x, y = torch.randn(64, 256, device="cuda"), torch.empty(64, 256, device="cuda")
     v, q, sc = torch.empty(300, device="cuda"), torch.empty(64, 256, dtype=torch.int8, device="cuda"), torch.empty(64, 2, device="cuda")
