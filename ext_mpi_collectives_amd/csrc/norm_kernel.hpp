@@ -775,7 +775,7 @@ int grad_w(const ext_mpi_amd_layernorm_grad &d, const grad_shape &s, float *part
   if (s.r.nv == 1) return grad_nv<T, W, 512, 1>(d, s, part, st);
   if (s.r.nv == 2) return grad_nv<T, W, 512, 2>(d, s, part, st);
   if (s.r.nv == 3) return grad_nv<T, W, 512, 3>(d, s, part, st);
-  if (s.r.nv == 4) return grad_nv<T, W, 512, 4>(d, s, part, st);
+  return grad_nv<T, W, 512, 4>(d, s, part, st);
 }
 
 template <class T>
