@@ -478,12 +478,16 @@ __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void laye
   grad_rows<T, W, MODE, NV, Q8, MULTI, TAIL, true>(d, blockIdx.x, gridDim.x, part);
 }
 
+// the sums of up to 512 lanes, by row taken and column
+template <int LANES>
+using lanes_sums = float[512 / LANES][8 * LANES];
+
 // The column sums alone: a workgroup takes 8 * LANES columns of every slices'th group of rows, as
 // many rows at a time as it has lanes for. `part` as in put_cols.
 template <class T, int LANES, bool Q8, bool MULTI, int TAIL>
-__device__ inline void cols_tile(const ext_mpi_amd_layernorm_grad &d, int tile, int slice, int slices, float *part) {
+__device__ inline void cols_tile(const ext_mpi_amd_layernorm_grad &d, int tile, int slice, int slices, float *part,
+                                 lanes_sums<LANES> *comb) {
   constexpr int C = 8 * LANES;
-  __shared__ float comb[2][512 / LANES][C]; // of up to 512 lanes
   const int l = threadIdx.x % LANES, k0 = threadIdx.x / LANES, R = blockDim.x / LANES;
   const int cols = (int)d.cols, nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
   const slot<TAIL> at(0, 0, tile * LANES + l, cols, true);
@@ -523,7 +527,8 @@ __device__ inline void cols_tile(const ext_mpi_amd_layernorm_grad &d, int tile, 
 // grid: slices (x), column tiles (y).
 template <class T, bool Q8>
 __global__ __launch_bounds__(256) void layernorm_cols_kernel(const ext_mpi_amd_layernorm_grad d, float *part) {
-  cols_tile<T, 64, Q8, true, WHOLE>(d, blockIdx.y, blockIdx.x, gridDim.x, part);
+  __shared__ lanes_sums<64> comb[2];
+  cols_tile<T, 64, Q8, true, WHOLE>(d, blockIdx.y, blockIdx.x, gridDim.x, part, comb);
 }
 
 // Rows without column sums, and in the workgroups behind theirs (from `blocks` on) the column sums of
@@ -532,17 +537,19 @@ __global__ __launch_bounds__(256) void layernorm_cols_kernel(const ext_mpi_amd_l
 template <class T, class W, int MODE, int NV, bool Q8, int TAIL>
 __global__ __launch_bounds__(lanes<MODE>::kBlock, lanes<MODE>::kWaves) void layernorm_grad_apart_kernel(
     const ext_mpi_amd_layernorm_grad d, int blocks) {
+  __shared__ lanes_sums<4> comb[2]; // one for all forms below
   if ((int)blockIdx.x < blocks) grad_rows<T, W, MODE, NV, Q8, true, TAIL, false>(d, blockIdx.x, blocks, nullptr);
-  else if (TAIL == PIECES) cols_tile<T, 4, Q8, true, PIECES>(d, blockIdx.x - blocks, 0, 1, nullptr);
-  else if (d.nsrc == 1) cols_tile<T, 4, Q8, false, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr);
-  else cols_tile<T, 4, Q8, true, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr);
+  else if (TAIL == PIECES) cols_tile<T, 4, Q8, true, PIECES>(d, blockIdx.x - blocks, 0, 1, nullptr, comb);
+  else if (d.nsrc == 1) cols_tile<T, 4, Q8, false, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr, comb);
+  else cols_tile<T, 4, Q8, true, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr, comb);
 }
 
 // Rows of more than 16384 columns. Held in registers they spill: a workgroup reads its row twice, for
 // the sums and for dx, the second time from the caches. The workgroups behind `blocks` as above.
 template <class T, class W, bool Q8>
 __global__ __launch_bounds__(512) void layernorm_grad_wide_kernel(const ext_mpi_amd_layernorm_grad d, int blocks) {
-  if ((int)blockIdx.x >= blocks) return cols_tile<T, 4, Q8, true, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr);
+  __shared__ lanes_sums<4> comb[2];
+  if ((int)blockIdx.x >= blocks) return cols_tile<T, 4, Q8, true, WHOLE>(d, blockIdx.x - blocks, 0, 1, nullptr, comb);
   const int cols = (int)d.cols, full = cols / 8, nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
   const float inv = 1.0f / (float)cols;
   __shared__ float red[2][lanes<512>::kSlots][2];
@@ -577,7 +584,6 @@ __global__ __launch_bounds__(512) void layernorm_grad_wide_kernel(const ext_mpi_
       }
     };
     const auto pass = [&](bool sums) {
-#pragma unroll 2
       for (int v = threadIdx.x; v < full; v += 512) take(slot<WHOLE>(0, 0, v, cols, true), sums, v);
       if (cols % 8 && (int)threadIdx.x == full % 512) take(slot<PIECES>(0, 0, full, cols, true), sums, full);
     };
