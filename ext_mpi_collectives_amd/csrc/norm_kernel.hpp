@@ -410,9 +410,11 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
       const slot<TAIL> at(i, per, l, cols, true);
       if (!MULTI) g[i] = widen<T>(ng[MULTI ? 0 : i]);
       g[i] = at.put(g[i]);
-      if (!ln.kOneRow && !live) g[i] = (f8)0.0f; // a row past the last
       xh[i] = nx[i].normed(rstd, shift, at);
       dsum[i] = nd[i];
+      // a row past the last, for which the last one was loaded: nothing of it counts, for its values may
+      // be infinite, or be replaced by dx in another wave at this time
+      if (!ln.kOneRow && !live) g[i] = xh[i] = (f8)0.0f;
     }
     if (AHEAD) load(within(row + step));
 #pragma unroll

@@ -707,3 +707,53 @@ def test_refusals_of_memory():
     h = act(64, 256, F, emac.SILU, ab.data_ptr(), ab[:, 256:].data_ptr(), a_stride=512, h_stride=512)
     emac.done(h)
     refused(ARG, act, 64, 256, F, emac.SILU, ab.data_ptr(), ab[:, 255:].data_ptr(), a_stride=512, h_stride=512)
+
+
+def gradient(dys, x, mean, rstd, dx=None, gt=torch.float32, **kw):
+    """dx (a new matrix unless given), dweight and dbias in type gt, of contiguous rows."""
+    rows, cols = x.shape
+    dx = torch.empty_like(x) if dx is None else dx
+    dw, db = torch.empty(cols, dtype=gt, device="cuda"), torch.empty(cols, dtype=gt, device="cuda")
+    go(emac.layernorm_grad_init(rows, cols, CODE[x.dtype], [d.data_ptr() for d in dys], mean.data_ptr(), rstd.data_ptr(), x=x.data_ptr(), dx=dx.data_ptr(),
+                                dweight=dw.data_ptr(), dbias=db.data_ptr(), gdtype=CODE[gt], **kw))
+    return dx, dw, db
+
+
+@pytest.mark.parametrize("nsrc", [1, 2])
+@pytest.mark.parametrize("rows,cols", [(300, 5), (300, 64), (1001, 131), (333, 200), (70001, 40), (1025, 512)])
+def test_rows_past_the_last_add_nothing(rows, cols, nsrc):
+    """Rows side by side in a workgroup that the last workgroup does not fill, and an infinity in the last
+    row: its column's sum is that infinity, all others are finite."""
+    gen = rnd(rows + cols)
+    x, dy = (torch.randn(rows, cols, device="cuda", generator=gen) for _ in range(2))
+    mean, rstd = x.mean(1), (x.var(1, unbiased=False) + 1e-5).rsqrt()
+    x[-1, 3], dy[-1, 3] = math.inf, 1.0
+    _, dw, db = gradient([dy] * nsrc, x, mean, rstd)
+    want = torch.zeros(cols, dtype=torch.bool, device="cuda")
+    want[3] = True
+    assert torch.equal(dw == math.inf, want) and torch.equal(dw.isfinite(), ~want) and bool(db.isfinite().all())
+
+
+@pytest.mark.parametrize("t", ["f16", "f32"])
+@pytest.mark.parametrize("nsrc", [1, 2])
+@pytest.mark.parametrize("rows,cols", [(5, 7), (29, 1024), (200, 300), (300, 5), (300, 64), (1001, 131), (333, 200), (70001, 40), (1025, 512), (700, 1000),
+                                       (600, 4099), (300, 9000), (9, 20001), (400, 20001)])
+def test_dx_over_x(rows, cols, nsrc, t):
+    """dx in place of x: the same bits as beside it, where the last row's dx overflows its type and dweight's
+    columns do not (fp16: g about 2^12 at an rstd of 2^9 gives 2^21 where 2^16 overflows; g xh is about 2^12 in
+    32 bits)."""
+    dt, gen = ref.TYPES[t], rnd(rows + cols + nsrc)
+    x = torch.randn(rows, cols, device="cuda", generator=gen).to(dt)
+    dys = [torch.randn(rows, cols, device="cuda", generator=gen).to(dt) for _ in range(nsrc)]
+    mean, rstd = x.float().mean(1), (x.float().var(1, unbiased=False) + 1e-5).rsqrt()
+    x[-1] /= 512
+    mean[-1], rstd[-1] = mean[-1] / 512, rstd[-1] * 512
+    dys[0][-1] *= 4096
+    kept = gradient(dys, x, mean, rstd)
+    x2 = x.clone()
+    over = gradient(dys, x2, mean, rstd, dx=x2)
+    if t == "f16":
+        assert bool(kept[0][-1].isinf().any())
+    assert bool(kept[1].isfinite().all()) and bool(kept[2].isfinite().all())
+    for a, b in zip(over, kept):
+        assert torch.equal(a, b)
