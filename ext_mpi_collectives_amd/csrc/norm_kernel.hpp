@@ -350,14 +350,11 @@ struct row8 {
       x = at.template load<T>(row_of<T>(d.x, row, d.x_stride));
     }
   }
-  // (x - mean) * rstd, as x * rstd - mean * rstd: two roundings of the products' size
-  __device__ f8 normed(float rstd, float shift, const slot<TAIL> &at) const {
-    if constexpr (Q8) {
-      const float s = scale * rstd;
-      return bytes(at.template put<signed char>(q)) * s + shift;
-    } else {
-      return widen<T>(at.template put<T>(x)) * rstd + shift;
-    }
+  // (x - mean) * rstd, the difference first: x * rstd - mean * rstd would be one operation, but off by half
+  // a step of mean * rstd, which is far more than xh in rows whose mean is large against their deviation
+  __device__ f8 normed(float mean, float rstd, const slot<TAIL> &at) const {
+    if constexpr (Q8) return (restore(at.template put<signed char>(q), scale) - mean) * rstd;
+    else return (widen<T>(at.template put<T>(x)) - mean) * rstd;
   }
 };
 
@@ -400,7 +397,7 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
     const long row = r0 + ln.sub;
     const bool live = ln.kOneRow || row < d.rows;
     if (!AHEAD) load(within(row));
-    const float rstd = nrstd, shift = -nmean * rstd;
+    const float rstd = nrstd, mean = nmean;
     f8 g[NV], xh[NV];
     raw8<T> dsum[NV];
     float s[2] = {0.0f, 0.0f};
@@ -410,7 +407,7 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
       const slot<TAIL> at(i, per, l, cols, true);
       if (!MULTI) g[i] = widen<T>(ng[MULTI ? 0 : i]);
       g[i] = at.put(g[i]);
-      xh[i] = nx[i].normed(rstd, shift, at);
+      xh[i] = nx[i].normed(mean, rstd, at);
       dsum[i] = nd[i];
       // a row past the last, for which the last one was loaded: nothing of it counts, for its values may
       // be infinite, or be replaced by dx in another wave at this time
@@ -503,7 +500,7 @@ __device__ inline void cols_tile(const ext_mpi_amd_layernorm_grad &d, int tile, 
     if (MULTI) fold_rows<T, 1, TAIL>(gs, d.dy, d.nsrc, row, d.dy_stride, 0, tile * LANES + l, cols);
     else gs[0] = widen<T>(at.template load<T>(row_of<T>(d.dy[0], row, d.dy_stride)));
     const f8 g = gs[0];
-    aw += g * x.normed(rstd, -mean * rstd, at);
+    aw += g * x.normed(mean, rstd, at);
     ab += g;
   }
 #pragma unroll
@@ -557,7 +554,7 @@ __global__ __launch_bounds__(512) void layernorm_grad_wide_kernel(const ext_mpi_
   __shared__ float red[2][lanes<512>::kSlots][2];
   row_sum<512, 2> sum_row(red);
   for (long row = blockIdx.x; row < d.rows; row += blocks) {
-    const float rstd = d.rstd[row], shift = -d.mean[row] * rstd;
+    const float rstd = d.rstd[row], mean = d.mean[row];
     float s[2] = {0.0f, 0.0f}, c1, c2;
     // vector v of the row: into the sums (and y), or into dx. Each lane loads its own elements alone,
     // which dx may replace.
@@ -570,7 +567,7 @@ __global__ __launch_bounds__(512) void layernorm_grad_wide_kernel(const ext_mpi_
       f8 g[1], ww = 1.0f;
       if (d.weight) ww = widen<W>(at.template load<W, true>(d.weight));
       fold_rows<T, 1, slot_t::kTail>(g, d.dy, d.nsrc, row, d.dy_stride, 0, v, cols);
-      const f8 xh = x.normed(rstd, shift, at);
+      const f8 xh = x.normed(mean, rstd, at);
       if (sums) {
         if (d.y) {
           f8 y = xh * ww;

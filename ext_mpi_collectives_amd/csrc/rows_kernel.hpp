@@ -346,7 +346,11 @@ __device__ inline f8 bytes(u2 q) {
   for (int j = 0; j < 8; j++) r[j] = (float)(int)(signed char)(q[j / 4] >> 8 * (j % 4));
   return r;
 }
-__device__ inline f8 restore(u2 q, float scale) { return bytes(q) * scale; }
+// what a checkpoint restores to, to the bit: the product is rounded on its own
+__device__ inline f8 restore(u2 q, float scale) {
+#pragma clang fp contract(off)
+  return bytes(q) * scale;
+}
 
 // A launch, with its own error and not one that an earlier call of the program left behind.
 template <class... A, class... V>

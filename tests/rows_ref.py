@@ -69,13 +69,16 @@ def stats_bounds(x, rstd):
     return 128 * U * big, 128 * U * (1 + rstd * big)
 
 
-def layernorm_grad(g, x, mean, rstd, w, dsum):
+def layernorm_grad(g, x, mean, rstd, w, dsum, exh=None):
     """In 64 bits, from 32-bit statistics: dx, dw, db and their bounds before they are rounded."""
     g, x, mean, rstd = g.double(), x.double(), mean.double()[:, None], rstd.double()[:, None]
     n, rows = x.shape[1], x.shape[0]
     w = torch.ones(n, dtype=torch.float64, device=x.device) if w is None else w.double()
     xh = (x - mean) * rstd
-    exh = 3 * U * (xh.abs() + rstd * (x.abs() + mean.abs()))  # of xh itself
+    if exh is None:  # of xh itself; or `exh` times its size
+        exh = 3 * U * (xh.abs() + rstd * (x.abs() + mean.abs()))
+    else:
+        exh = exh * xh.abs()
     gw = g * w
     c1, c2 = gw.mean(1, keepdim=True), (gw * xh).mean(1, keepdim=True)
     dx = rstd * (gw - c1 - xh * c2)

@@ -757,3 +757,37 @@ def test_dx_over_x(rows, cols, nsrc, t):
     assert bool(kept[1].isfinite().all()) and bool(kept[2].isfinite().all())
     for a, b in zip(over, kept):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("nsrc", [1, 2])
+@pytest.mark.parametrize("rows,cols", [(20, 5), (300, 7), (40, 100), (600, 100), (50, 129), (500, 500), (30, 1024), (600, 1027), (500, 5000), (400, 9001),
+                                       (300, 13000), (8, 20001), (300, 20001)])
+def test_rows_with_a_large_mean(rows, cols, nsrc, t):
+    """Rows a thousand deviations from zero. (x - mean) * rstd is off by a rounding of the difference and one of the
+    product, 2 U of its own size (3 U are counted): no rounding is of the size of x or of mean * rstd. From a checkpoint too,
+    whose restored values are fixed to the bit."""
+    dt, gen = ref.TYPES[t], rnd(rows + cols)
+    x = (torch.randn(rows, cols, device="cuda", generator=gen) + 1000).to(dt)
+    dys = [torch.randn(rows, cols, device="cuda", generator=gen).to(dt) for _ in range(nsrc)]
+    w = torch.randn(cols, device="cuda", generator=gen)
+    y, mean, rstd = torch.empty_like(x), torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    q, scale = torch.empty(rows, cols, dtype=torch.int8, device="cuda"), torch.empty(rows, -(-cols // 128), device="cuda")
+    go(emac.layernorm_init(rows, cols, CODE[dt], [x.data_ptr()], y.data_ptr(), weight=w.data_ptr(), wdtype=emac.FLOAT, mean=mean.data_ptr(),
+                           rstd=rstd.data_ptr(), q=q.data_ptr(), scale=scale.data_ptr()))
+    rmean, _, ry, by = ref.layernorm(x, w, None, 1e-5)
+    ref.close(y, ry, by)
+    ref.close(mean, rmean, ref.stats_bounds(x, rstd.double())[0])
+    rq, rscale = ref.save8(x)
+    assert torch.equal(q, rq) and torch.equal(scale, rscale)
+    g = dys[0].float()
+    for d in dys[1:]:
+        g = g + d.float()
+    for xv, kw in ((x, {"x": x.data_ptr()}), (ref.restore8(rq, rscale), {"q": q.data_ptr(), "scale": scale.data_ptr()})):
+        dx, dw, db = torch.empty_like(x), torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+        go(emac.layernorm_grad_init(rows, cols, CODE[dt], [d.data_ptr() for d in dys], mean.data_ptr(), rstd.data_ptr(), dx=dx.data_ptr(),
+                                    dweight=dw.data_ptr(), dbias=db.data_ptr(), weight=w.data_ptr(), wdtype=emac.FLOAT, gdtype=emac.FLOAT, **kw))
+        rdx, bdx, rdw, bdw, rdb, bdb = ref.layernorm_grad(g, xv, mean, rstd, w, None, exh=3 * ref.U)
+        ref.close(dx, rdx, bdx)
+        ref.close(dw, rdw, bdw)
+        ref.close(db, rdb, bdb)
