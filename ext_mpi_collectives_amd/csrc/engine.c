@@ -453,7 +453,7 @@ int ext_mpi_amd_test(int handle) {
   int rc;
   if (!h) return EMAC_ERR_ARG;
   if (!h->started) return 1;
-  rc = emac_gpu_stream_query(h->stream);
+  rc = h->rows ? rows_query(h) : emac_gpu_stream_query(h->stream);
   if (rc == 1) {
     h->started = 0;
     if (ipc_status(h)) return EMAC_ERR_TRANSPORT;
@@ -466,7 +466,7 @@ int ext_mpi_amd_wait(int handle) {
   int rc;
   if (!h) return EMAC_ERR_ARG;
   if (h->rows && !h->started) return 0;
-  rc = emac_gpu_stream_sync(h->stream);
+  rc = h->rows ? rows_sync(h) : emac_gpu_stream_sync(h->stream);
   h->started = 0;
   return rc ? rc : ipc_status(h);
 }

@@ -315,6 +315,8 @@ int stage_out(emac_handle *h);
 int rows_stream(emac_handle *h);
 int rows_set_stream(emac_handle *h, void *stream);
 int rows_start(emac_handle *h);
+int rows_sync(emac_handle *h);
+int rows_query(emac_handle *h);
 void rows_free(emac_handle *h);
 
 /* engine_tune.c */

@@ -354,8 +354,21 @@ int rows_stream(emac_handle *h) {
   return rc;
 }
 
+/* f of the handle's stream with the handle's device current: the default stream is the current device's */
+static int on_device(emac_handle *h, int (*f)(void *)) {
+  int cur = -1, rc;
+  emac_gpu_get_device(&cur);
+  if (cur != h->device && emac_gpu_set_device(h->device)) return EMAC_ERR_DEVICE;
+  rc = f(h->stream);
+  if (cur >= 0 && cur != h->device) emac_gpu_set_device(cur);
+  return rc;
+}
+
+int rows_sync(emac_handle *h) { return on_device(h, emac_gpu_stream_sync); }
+int rows_query(emac_handle *h) { return on_device(h, emac_gpu_stream_query); }
+
 int rows_set_stream(emac_handle *h, void *stream) {
-  if (h->started && emac_gpu_stream_sync(h->stream)) return EMAC_ERR_DEVICE;
+  if (h->started && rows_sync(h)) return EMAC_ERR_DEVICE;
   h->started = 0;
   if (h->own_stream && h->stream) emac_gpu_stream_destroy(h->stream);
   h->stream = stream;
@@ -388,7 +401,7 @@ int rows_start(emac_handle *h) {
 
 void rows_free(emac_handle *h) {
   if (!h->rows) return;
-  if (h->started) emac_gpu_stream_sync(h->stream); /* the default stream too */
+  if (h->started) rows_sync(h); /* the default stream too */
   emac_gpu_free(h->rows->ws);
   free(h->rows);
   h->rows = NULL;

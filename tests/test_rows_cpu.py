@@ -2,6 +2,8 @@
 matrices for shared bytes, and the oracle's own checkpoint against the definition in 64 bits."""
 import ctypes
 import math
+import os
+import subprocess
 
 import pytest
 import torch
@@ -112,3 +114,23 @@ def test_struct_layouts():
     assert ctypes.sizeof(emac.LayernormGradDesc) == 16 + 24 + 16 * 8 + 18 * 8
     assert ctypes.sizeof(emac.ActDesc) == 24 + 11 * 8
     assert ctypes.sizeof(emac.ActGradDesc) == 24 + 13 * 8
+
+
+@pytest.fixture(scope="module")
+def host_check(tmp_path_factory):
+    """tests/rows_host_check.c over the engine's own sources."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    src, exe = os.path.join(here, "..", "ext_mpi_collectives_amd", "csrc"), str(tmp_path_factory.mktemp("rows") / "check")
+    units = [os.path.join(src, f"{u}.c") for u in ("engine", "engine_rows", "engine_tune", "engine_node", "engine_comm", "engine_ipc", "engine_join", "plan", "layout")]
+    subprocess.run(["gcc", "-O1", "-g", "-std=gnu11", "-w", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I" + os.path.join(src, "..", "..", "include"), "-I" + src,
+                    "-o", exe, os.path.join(here, "rows_host_check.c"), *units, "-no-pie", "-Wl,--unresolved-symbols=ignore-all"], check=True)
+
+    def run(what):
+        r = subprocess.run([exe, what], capture_output=True, text=True, timeout=60)
+        assert r.returncode == 0, r.stdout + r.stderr
+    return run
+
+
+def test_the_default_stream_of_another_device(host_check):
+    """Start, Test, Wait, set_stream and Done of a handle on its device's default stream, another device current."""
+    host_check("default_stream")
