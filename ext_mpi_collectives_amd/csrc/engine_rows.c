@@ -27,6 +27,7 @@ struct emac_rows {
   } d;
   void *ws;       /* the gradient's partial rows */
   int stream_set; /* the caller's stream, which may be NULL (the default stream) */
+  int anywhere;   /* no memory (no rows): any device will do */
 };
 
 /* ---- the memory a descriptor names ---- */
@@ -184,7 +185,8 @@ static int finish(const memory *m, int what, const void *d, size_t bytes, size_t
   h->rows->what = what;
   memcpy(&h->rows->d, d, bytes);
   emac_gpu_get_device(&cur);
-  h->device = m->device >= 0 ? m->device : cur;
+  h->rows->anywhere = m->device < 0;
+  h->device = h->rows->anywhere ? cur : m->device;
   if (ws) {
     rc = emac_gpu_set_device(h->device);
     if (!rc) rc = emac_gpu_malloc(&h->rows->ws, ws);
@@ -354,20 +356,29 @@ int rows_stream(emac_handle *h) {
   return rc;
 }
 
-/* f of the handle's stream with the handle's device current: the default stream is the current device's */
-static int on_device(emac_handle *h, int (*f)(void *)) {
+/* f of a stream with the handle's device current: the default stream is the current device's */
+static int on_device(const emac_handle *h, void *stream, int (*f)(void *)) {
   int cur = -1, rc;
   emac_gpu_get_device(&cur);
   if (cur != h->device && emac_gpu_set_device(h->device)) return EMAC_ERR_DEVICE;
-  rc = f(h->stream);
+  rc = f(stream);
   if (cur >= 0 && cur != h->device) emac_gpu_set_device(cur);
   return rc;
 }
 
-int rows_sync(emac_handle *h) { return on_device(h, emac_gpu_stream_sync); }
-int rows_query(emac_handle *h) { return on_device(h, emac_gpu_stream_query); }
+int rows_sync(emac_handle *h) { return on_device(h, h->stream, emac_gpu_stream_sync); }
+int rows_query(emac_handle *h) { return on_device(h, h->stream, emac_gpu_stream_query); }
+
+/* whether a stream is the current device's */
+static int stream_here(void *stream) {
+  int dev, cur;
+  if (emac_gpu_stream_device(stream, &dev)) return EMAC_ERR_ARG;
+  return emac_gpu_get_device(&cur) || dev != cur ? EMAC_ERR_ARG : 0;
+}
 
 int rows_set_stream(emac_handle *h, void *stream) {
+  const int rc = h->rows->anywhere ? 0 : on_device(h, stream, stream_here);
+  if (rc) return rc;
   if (h->started && rows_sync(h)) return EMAC_ERR_DEVICE;
   h->started = 0;
   if (h->own_stream && h->stream) emac_gpu_stream_destroy(h->stream);

@@ -287,6 +287,17 @@ int emac_gpu_stream_query(void *stream) {
   }
   return EMAC_ERR_DEVICE;
 }
+int emac_gpu_stream_device(void *stream, int *dev) {
+  hipDevice_t d;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (!s || s == hipStreamPerThread || s == hipStreamLegacy) return ok(hipGetDevice(dev));
+  if (hipStreamGetDevice(s, &d) != hipSuccess) {
+    clear_error("emac_gpu_stream_device");
+    return EMAC_ERR_ARG;
+  }
+  *dev = d;
+  return 0;
+}
 int emac_gpu_device_sync(void) { return ok(hipDeviceSynchronize()); }
 int emac_gpu_event_create(void **ev) {
   hipEvent_t e;

@@ -61,6 +61,7 @@ int emac_gpu_stream_create(void **stream);
 int emac_gpu_stream_destroy(void *stream);
 int emac_gpu_stream_sync(void *stream);
 int emac_gpu_stream_query(void *stream); /* 1 idle, 0 busy, <0 error */
+int emac_gpu_stream_device(void *stream, int *dev); /* a stream's own; a default stream has the current one */
 int emac_gpu_device_sync(void);
 int emac_gpu_event_create(void **ev); /* timing disabled */
 int emac_gpu_event_create_timed(void **ev);

@@ -117,9 +117,10 @@ int ext_mpi_amd_comm_mfree(int comm, void *p);
  * (ext_mpi_amd_start / _test / _wait / _done); one Start of a handle is in flight at a time (a
  * gradient handle owns a workspace), also across graphs that captured its Start; such a graph must
  * not be replayed after Done, and the stream to capture on is set (ext_mpi_amd_set_stream) before
- * the capture begins. set_stream also takes the default stream (NULL) here, and Start leaves the
- * caller's current device as it was. No Start allocates or waits (the first one on a handle without
- * a stream set creates the handle's own).
+ * the capture begins. set_stream also takes the default stream (NULL) here, and refuses a stream of
+ * another device than the memory's with EXT_MPI_AMD_ERROR_ARG (the handle keeps the one it had);
+ * Start leaves the caller's current device as it was. No Start allocates or waits (the first one on
+ * a handle without a stream set creates the handle's own).
  * An output may be one of the inputs of the same type, in place (same address and stride), except
  * layernorm_grad's y; any other overlap with an output is EXT_MPI_AMD_ERROR_ARG, as are negative
  * sizes, short strides, misaligned, host or foreign-device pointers. */

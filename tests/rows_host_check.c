@@ -20,6 +20,7 @@ int emac_gpu_stream_create(void **s) { *s = malloc(1); live_streams++; return 0;
 int emac_gpu_stream_destroy(void *s) { free(s); live_streams--; return 0; }
 int emac_gpu_stream_sync(void *s) { synced = s ? 100 : current; return 0; }
 int emac_gpu_stream_query(void *s) { queried = s ? 100 : current; return 0; }
+int emac_gpu_stream_device(void *s, int *d) { *d = s ? (int)((size_t)s >> 28) : current; return 0; }
 int emac_gpu_event_destroy(void *e) { return 0; }
 int emac_gpu_graph_destroy(void *g) { return 0; }
 int emac_gpu_act(const ext_mpi_amd_act *d, void *s) { launched = current; return 0; }
@@ -60,9 +61,24 @@ static void default_stream_of_another_device(void) {
   CHECK(ext_mpi_amd_done(h) == 0 && synced == 1 && current == 0);
 }
 
+/* memory and stream of one device, whichever is current */
+static void stream_of_another_device(void) {
+  int h = save8(1);
+  synced = -1;
+  CHECK(ext_mpi_amd_set_stream(h, ON(1, 7)) == 0);
+  CHECK(ext_mpi_amd_start(h) == 0 && launched == 1);
+  CHECK(ext_mpi_amd_set_stream(h, ON(0, 7)) == EXT_MPI_AMD_ERROR_ARG && synced == -1);
+  CHECK(ext_mpi_amd_stream(h) == ON(1, 7)); /* as before */
+  CHECK(ext_mpi_amd_set_stream(h, NULL) == 0 && current == 0);
+  CHECK(ext_mpi_amd_done(h) == 0);
+  CHECK(ext_mpi_amd_save8_init(0, 8, EXT_MPI_AMD_FLOAT, NULL, 0, NULL, 0, NULL, &h) == 0); /* no rows, no memory */
+  CHECK(ext_mpi_amd_set_stream(h, ON(1, 7)) == 0 && ext_mpi_amd_start(h) == 0 && ext_mpi_amd_done(h) == 0);
+}
+
 int main(int argc, char **argv) {
   const char *what = argc > 1 ? argv[1] : "";
   if (!strcmp(what, "default_stream")) default_stream_of_another_device();
+  else if (!strcmp(what, "other_stream")) stream_of_another_device();
   else return 2;
   CHECK(live_streams == 0);
   return 0;

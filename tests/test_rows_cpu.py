@@ -134,3 +134,8 @@ def host_check(tmp_path_factory):
 def test_the_default_stream_of_another_device(host_check):
     """Start, Test, Wait, set_stream and Done of a handle on its device's default stream, another device current."""
     host_check("default_stream")
+
+
+def test_a_stream_of_another_device_is_refused(host_check):
+    """The handle keeps the stream it had."""
+    host_check("other_stream")
