@@ -206,7 +206,9 @@ int ext_mpi_amd_layernorm_init(const ext_mpi_amd_layernorm *desc, int *handle) {
   if (!desc || !handle) return EMAC_ERR_ARG;
   d = *desc;
   if ((rc = begin(&m, d.rows, d.cols, EXT_MPI_AMD_ROW_COLS_MAX, d.dtype, handle))) return rc;
-  if (d.nsrc < 1 || d.nsrc > EMAC_MAX_RANKS || !(d.eps >= 0.0) || isinf(d.eps)) return EMAC_ERR_ARG;
+  if (d.nsrc < 1 || d.nsrc > EMAC_MAX_RANKS) return EMAC_ERR_ARG;
+  /* the kernels add it as a float: 0 in place of a smaller eps would make a row of one value NaN */
+  if (!(d.eps >= 0.0) || isinf((float)d.eps) || (d.eps > 0.0 && (float)d.eps == 0.0f)) return EMAC_ERR_ARG;
   if (!d.y && !d.sum && !d.q && d.rows > 0) return EMAC_ERR_ARG;
   if ((d.weight || d.bias) && (rc = type2_check(d.wdtype, d.dtype))) return rc;
   es = elem_size(d.dtype);

@@ -148,7 +148,7 @@ typedef struct {
   const void *residual; /* optional */
   long residual_stride;
   const void *weight, *bias; /* cols elements; optional (1 and 0) */
-  double eps;
+  double eps;        /* 0, or in a float's range (about 1e-45 to 3.4e38) */
   void *y;           /* optional if sum or q is given */
   long y_stride;
   void *sum;         /* optional: x */

@@ -75,10 +75,33 @@ static void stream_of_another_device(void) {
   CHECK(ext_mpi_amd_set_stream(h, ON(1, 7)) == 0 && ext_mpi_amd_start(h) == 0 && ext_mpi_amd_done(h) == 0);
 }
 
+/* eps is added as a float: 0, or what a float holds */
+static void eps_range(void) {
+  const double in[] = {0.0, 1.5e-45, 1e-38, 1e-5, 3.4e38}, out[] = {-1.0, -1e-60, 1e-60, 7e-46, 3.5e38, 1e300, 1.0 / 0.0, 0.0 / 0.0};
+  ext_mpi_amd_layernorm d = {0};
+  unsigned k;
+  int h;
+  d.rows = 2;
+  d.cols = 8;
+  d.dtype = EXT_MPI_AMD_FLOAT;
+  d.nsrc = 1;
+  d.src[0] = ON(0, 1);
+  d.y = ON(0, 2);
+  for (k = 0; k < sizeof(in) / sizeof(*in); k++) {
+    d.eps = in[k];
+    CHECK(ext_mpi_amd_layernorm_init(&d, &h) == 0 && ext_mpi_amd_done(h) == 0);
+  }
+  for (k = 0; k < sizeof(out) / sizeof(*out); k++) {
+    d.eps = out[k];
+    CHECK(ext_mpi_amd_layernorm_init(&d, &h) == EXT_MPI_AMD_ERROR_ARG);
+  }
+}
+
 int main(int argc, char **argv) {
   const char *what = argc > 1 ? argv[1] : "";
   if (!strcmp(what, "default_stream")) default_stream_of_another_device();
   else if (!strcmp(what, "other_stream")) stream_of_another_device();
+  else if (!strcmp(what, "eps")) eps_range();
   else return 2;
   CHECK(live_streams == 0);
   return 0;

@@ -139,3 +139,8 @@ def test_the_default_stream_of_another_device(host_check):
 def test_a_stream_of_another_device_is_refused(host_check):
     """The handle keeps the stream it had."""
     host_check("other_stream")
+
+
+def test_eps_is_a_floats(host_check):
+    """An eps that a float takes for 0 or for an infinity is refused, like a negative one."""
+    host_check("eps")
