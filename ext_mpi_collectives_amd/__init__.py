@@ -55,6 +55,7 @@ _ipc_callbacks = {}  # comm -> the ctypes callback (must outlive the communicato
 SILU, GELU, GELU_TANH = 0, 1, 2  # include/ext_mpi_amd.h EXT_MPI_AMD_SILU / _GELU / _GELU_TANH
 BLOCK8 = 128            # columns that share a checkpoint's scale
 ROW_COLS_MAX = 65536    # layer norm: columns
+COLS8_MAX, BLOCKS8_MAX = 1 << 30, (1 << 31) - 4096  # checkpoints and activations: columns, rows * ceil(cols / 128)
 _P, _L, _I = ctypes.c_void_p, ctypes.c_long, ctypes.c_int
 _LEAVES = ctypes.c_void_p * MAX_RANKS
 

@@ -144,24 +144,24 @@ static int settle(memory *m) {
   return m->rc;
 }
 
-static int begin(memory *m, long rows, long cols, long most, int dtype, int *handle) {
+/* The kernels of act8.hip number columns and checkpoint blocks in 32 bits (narrow matrices of a device's
+   memory can have more blocks: 2^31 of one bf16 column are 15 GB with their checkpoint); the last 4096 of
+   them are left for a launch's own rounding up. */
+static int fits8(long rows, long cols) {
+  if (cols < 1 || cols > EXT_MPI_AMD_COLS8_MAX) return 0;
+  return rows <= EXT_MPI_AMD_BLOCKS8_MAX / ((cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8);
+}
+
+static int begin(memory *m, long rows, long cols, int fits, int dtype, int *handle) {
   int rc;
   memset(m, 0, sizeof(*m));
   m->device = -1;
   *handle = -1;
   if (rows < 0 || cols < 1) return EMAC_ERR_ARG;
   if ((rc = type_check(dtype))) return rc;
-  if (cols > most) return EMAC_ERR_UNSUPPORTED;
+  if (!fits) return EMAC_ERR_UNSUPPORTED;
   if (emac_gpu_device_count() <= 0) return EMAC_ERR_DEVICE;
   return 0;
-}
-
-/* checkpoint blocks are numbered in 32 bits by the kernels of act8.hip (2^31 of them are more
-   than the memory of a device) */
-#define COLS8_MAX (1L << 30)
-static int blocks_fit(long rows, long cols) {
-  const long nblk = (cols + EMAC_BLOCK8 - 1) / EMAC_BLOCK8;
-  return rows <= ((1L << 31) - 4096) / nblk;
 }
 
 static void add_saved(memory *m, long rows, long cols, const signed char *q, long *q_stride, const float *scale, int out,
@@ -205,7 +205,7 @@ int ext_mpi_amd_layernorm_init(const ext_mpi_amd_layernorm *desc, int *handle) {
   int rc, i, es;
   if (!desc || !handle) return EMAC_ERR_ARG;
   d = *desc;
-  if ((rc = begin(&m, d.rows, d.cols, EXT_MPI_AMD_ROW_COLS_MAX, d.dtype, handle))) return rc;
+  if ((rc = begin(&m, d.rows, d.cols, d.cols <= EXT_MPI_AMD_ROW_COLS_MAX, d.dtype, handle))) return rc;
   if (d.nsrc < 1 || d.nsrc > EMAC_MAX_RANKS) return EMAC_ERR_ARG;
   /* the kernels add it as a float: 0 in place of a smaller eps would make a row of one value NaN */
   if (!(d.eps >= 0.0) || isinf((float)d.eps) || (d.eps > 0.0 && (float)d.eps == 0.0f)) return EMAC_ERR_ARG;
@@ -231,7 +231,7 @@ int ext_mpi_amd_layernorm_grad_init(const ext_mpi_amd_layernorm_grad *desc, int 
   int rc, i, es;
   if (!desc || !handle) return EMAC_ERR_ARG;
   d = *desc;
-  if ((rc = begin(&m, d.rows, d.cols, EXT_MPI_AMD_ROW_COLS_MAX, d.dtype, handle))) return rc;
+  if ((rc = begin(&m, d.rows, d.cols, d.cols <= EXT_MPI_AMD_ROW_COLS_MAX, d.dtype, handle))) return rc;
   if (d.nsrc < 1 || d.nsrc > EMAC_MAX_RANKS) return EMAC_ERR_ARG;
   if (!d.dx && !d.dweight && !d.dbias && d.rows > 0) return EMAC_ERR_ARG;
   if (d.rows > 0 && !d.x == !d.q) return EMAC_ERR_ARG; /* exactly one */
@@ -261,8 +261,7 @@ int ext_mpi_amd_save8_init(long rows, long cols, int dtype, const void *x, long 
   memory m;
   int rc;
   if (!handle) return EMAC_ERR_ARG;
-  if ((rc = begin(&m, rows, cols, COLS8_MAX, dtype, handle))) return rc;
-  if (!blocks_fit(rows, cols)) return EMAC_ERR_UNSUPPORTED;
+  if ((rc = begin(&m, rows, cols, fits8(rows, cols), dtype, handle))) return rc;
   add(&m, x, rows, cols, &x_stride, elem_size(dtype), -1, 0, 0);
   add_saved(&m, rows, cols, q, &q_stride, scale, 1, 0);
   if ((rc = settle(&m))) return rc;
@@ -285,8 +284,7 @@ int ext_mpi_amd_restore8_init(long rows, long cols, int dtype, const signed char
   memory m;
   int rc;
   if (!handle) return EMAC_ERR_ARG;
-  if ((rc = begin(&m, rows, cols, COLS8_MAX, dtype, handle))) return rc;
-  if (!blocks_fit(rows, cols)) return EMAC_ERR_UNSUPPORTED;
+  if ((rc = begin(&m, rows, cols, fits8(rows, cols), dtype, handle))) return rc;
   add_saved(&m, rows, cols, q, &q_stride, scale, 0, 0);
   add(&m, x, rows, cols, &x_stride, elem_size(dtype), -1, 1, 0);
   if ((rc = settle(&m))) return rc;
@@ -308,9 +306,8 @@ int ext_mpi_amd_act_init(const ext_mpi_amd_act *desc, int *handle) {
   int rc, es;
   if (!desc || !handle) return EMAC_ERR_ARG;
   d = *desc;
-  if ((rc = begin(&m, d.rows, d.cols, COLS8_MAX, d.dtype, handle))) return rc;
+  if ((rc = begin(&m, d.rows, d.cols, fits8(d.rows, d.cols), d.dtype, handle))) return rc;
   if (d.kind < EXT_MPI_AMD_SILU || d.kind > EXT_MPI_AMD_GELU_TANH) return EMAC_ERR_ARG;
-  if (!blocks_fit(d.rows, d.cols)) return EMAC_ERR_UNSUPPORTED;
   if (!d.h && !d.qa && d.rows > 0) return EMAC_ERR_ARG;
   /* the gate's checkpoint goes with the gate's and the other's */
   if (d.rows > 0 && !d.qb != !(d.b && d.qa)) return EMAC_ERR_ARG;
@@ -330,9 +327,8 @@ int ext_mpi_amd_act_grad_init(const ext_mpi_amd_act_grad *desc, int *handle) {
   int rc, es;
   if (!desc || !handle) return EMAC_ERR_ARG;
   d = *desc;
-  if ((rc = begin(&m, d.rows, d.cols, COLS8_MAX, d.dtype, handle))) return rc;
+  if ((rc = begin(&m, d.rows, d.cols, fits8(d.rows, d.cols), d.dtype, handle))) return rc;
   if (d.kind < EXT_MPI_AMD_SILU || d.kind > EXT_MPI_AMD_GELU_TANH) return EMAC_ERR_ARG;
-  if (!blocks_fit(d.rows, d.cols)) return EMAC_ERR_UNSUPPORTED;
   if (d.rows > 0 && !d.qb != !d.db) return EMAC_ERR_ARG; /* a gate and its gradient */
   es = elem_size(d.dtype);
   add(&m, d.dh, d.rows, d.cols, &d.dh_stride, es, d.dtype, 0, 0);

@@ -128,6 +128,9 @@ int ext_mpi_amd_comm_mfree(int comm, void *p);
 #define EXT_MPI_AMD_HALF 5
 #define EXT_MPI_AMD_ROW_COLS_MAX 65536 /* layer norm: columns (above: EXT_MPI_AMD_ERROR_UNSUPPORTED) */
 #define EXT_MPI_AMD_BLOCK8 128         /* columns that share a checkpoint's scale */
+/* save8, restore8, act and act_grad: columns, and rows times ceil(cols / 128) (above: EXT_MPI_AMD_ERROR_UNSUPPORTED) */
+#define EXT_MPI_AMD_COLS8_MAX (1L << 30)
+#define EXT_MPI_AMD_BLOCKS8_MAX ((1L << 31) - 4096)
 
 /* A checkpoint of a rows x cols matrix: q, rows x cols signed bytes (row stride q_stride >= cols, 0:
  * cols), and scale, rows x ceil(cols / 128) floats, contiguous. For each block of 128 columns,

@@ -791,3 +791,16 @@ def test_rows_with_a_large_mean(rows, cols, nsrc, t):
         ref.close(dx, rdx, bdx)
         ref.close(dw, rdw, bdw)
         ref.close(db, rdb, bdb)
+
+
+def test_the_most_blocks():
+    """As many blocks as are taken, of one column each."""
+    rows = emac.BLOCKS8_MAX
+    x = torch.randint(0, 2, (rows, 1), dtype=torch.int8, device="cuda", generator=rnd(9)).mul_(2).sub_(1)
+    t = x.to(torch.bfloat16)
+    q, scale = torch.empty(rows, 1, dtype=torch.int8, device="cuda"), torch.empty(rows, 1, device="cuda")
+    go(emac.save8_init(rows, 1, emac.BF16, t.data_ptr(), q.data_ptr(), scale.data_ptr()))
+    assert torch.equal(q, x.mul_(127))
+    t.zero_()
+    go(emac.restore8_init(rows, 1, emac.BF16, q.data_ptr(), scale.data_ptr(), t.data_ptr()))
+    assert torch.equal(t.to(torch.int8).mul_(127), x)

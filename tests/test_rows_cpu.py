@@ -144,3 +144,18 @@ def test_a_stream_of_another_device_is_refused(host_check):
 def test_eps_is_a_floats(host_check):
     """An eps that a float takes for 0 or for an infinity is refused, like a negative one."""
     host_check("eps")
+
+
+@pytest.mark.parametrize("call", range(2, len(CALLS)))
+def test_the_most_columns_and_blocks(call):
+    """Checkpoints and activations: the header's limits are the last sizes that are not refused as too large."""
+    f, t = CALLS[call], emac.FLOAT
+    text = open(os.path.join(os.path.dirname(emac.HERE), "include", "ext_mpi_amd.h")).read()
+    assert "#define EXT_MPI_AMD_COLS8_MAX (1L << 30)" in text and "#define EXT_MPI_AMD_BLOCKS8_MAX ((1L << 31) - 4096)" in text
+    assert (emac.COLS8_MAX, emac.BLOCKS8_MAX) == (1 << 30, (1 << 31) - 4096)
+    for cols in (1, 127, 128, 129, 1000, emac.COLS8_MAX):
+        most = emac.BLOCKS8_MAX // -(-cols // 128)
+        assert code_of(f, most + 1, cols, t) == UNSUPPORTED
+        assert code_of(f, 1 << 40, cols, t) == UNSUPPORTED
+        assert code_of(f, most, cols, t) != UNSUPPORTED  # no device, or no memory at the addresses
+    assert code_of(f, 1, emac.COLS8_MAX + 1, t) == UNSUPPORTED
