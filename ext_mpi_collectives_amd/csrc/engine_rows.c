@@ -130,6 +130,12 @@ int ext_mpi_amd_check_rows_share(long a, long rows_a, long len_a, long ld_a, lon
   return share(&x, &y);
 }
 
+/* the polynomial of the normal distribution's tail for tests (host only): its argument's factor, its coefficients */
+double ext_mpi_amd_check_gelu_tail(int k) {
+  static const float c[8] = EMAC_GELU_TAIL;
+  return k ? c[(k - 1) & 7] : EMAC_GELU_TAIL_AT;
+}
+
 static int settle(memory *m) {
   int i, k;
   for (i = 0; i < m->n && !m->rc; i++)

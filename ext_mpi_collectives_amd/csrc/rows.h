@@ -15,6 +15,13 @@ extern "C" {
 
 #define EMAC_BLOCK8 EXT_MPI_AMD_BLOCK8
 
+/* erfcx(z) / 2 for z = |a| / sqrt 2 as a polynomial of degree 8 in t = 1 / (1 + 0.4348731 z) = 1 / (1 + AT |a|)
+   without a constant term, the highest power first; fitted for the least relative error on 0 <= z <= 12 */
+#define EMAC_GELU_TAIL_AT 0.30750170f
+#define EMAC_GELU_TAIL                                                                                      \
+  {0.036300003528594971f, -0.14733710885047913f, 0.1701858937740326f, -0.026046559214591980f,             \
+   0.1153081208467484f,   0.1056915521621704f,   0.1232480555772781f, 0.1226501166820526f}
+
 /* layer norm, forward: one launch */
 int emac_gpu_layernorm(const ext_mpi_amd_layernorm *d, void *stream);
 /* its gradient: one to three launches; `part` is the workspace of emac_gpu_layernorm_grad_ws bytes */
