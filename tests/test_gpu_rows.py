@@ -1,6 +1,8 @@
 """The row operators on the GPU against their definitions in 64 bits (tests/rows_ref.py): layer norm over
 folded leaves, its gradient, checkpoints in 8 bits, activations and their gradient."""
+import importlib.util
 import math
+import os
 
 import pytest
 import torch
@@ -804,3 +806,106 @@ def test_the_most_blocks():
     t.zero_()
     go(emac.restore8_init(rows, 1, emac.BF16, q.data_ptr(), scale.data_ptr(), t.data_ptr()))
     assert torch.equal(t.to(torch.int8).mul_(127), x)
+
+
+@pytest.mark.parametrize("name", ["norm_prefill", "grad_batch"])
+def test_a_pass_of_the_cases_follows_the_current_stream(name):
+    """perf/operators.py: handles prepared on one stream, a pass under another, behind a late producer of its inputs."""
+    spec = importlib.util.spec_from_file_location("operators_own", os.path.join(os.path.dirname(emac.HERE), "perf", "operators.py"))
+    ops = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ops)
+    ops.own = True
+    state = ops.prepare(next(c for c in ops.listed() if c["name"] == name), 1)
+    want = {k: v.clone() for k, v in ops.run(state).items()}
+    src = state["in"]["src" if name == "norm_prefill" else "dy"][0]
+    kept = src.clone()
+    src.zero_()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(200_000_000)
+        src.copy_(kept)
+        got = {k: v.clone() for k, v in ops.run(state).items()}
+    s.synchronize()
+    for k in want:
+        assert torch.equal(got[k], want[k])
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("w32", [False, True])
+@pytest.mark.parametrize("rows,cols", WIDTHS)
+def test_one_leaf_over_many_rows(rows, cols, w32, t):
+    """One leaf, more rows than workgroups, against the definitions: the norm with a residual (and without weights, one
+    leaf alone), its gradient with dsum from x and from the checkpoint, without the norm's output again."""
+    dt, gen = ref.TYPES[t], rnd(rows + cols + w32)
+    wt = torch.float32 if w32 else dt
+    src, res, dy, dsum = (torch.randn(rows, cols, device="cuda", generator=gen).to(dt) for _ in range(4))
+    w, b = (torch.randn(cols, device="cuda", generator=gen).to(wt) for _ in range(2))
+    x, y = torch.empty_like(src), torch.empty_like(src)
+    mean, rstd = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    kw = dict(mean=mean.data_ptr(), rstd=rstd.data_ptr())
+    for r in (None, res):
+        ww, bb = (None, None) if r is None else (w, b)
+        more = {} if r is None else dict(residual=r.data_ptr(), sum=x.data_ptr(), weight=w.data_ptr(), bias=b.data_ptr(), wdtype=CODE[wt])
+        go(emac.layernorm_init(rows, cols, CODE[dt], [src.data_ptr()], y.data_ptr(), **kw, **more))
+        want = ref.fold([src], r)
+        assert r is None or torch.equal(x, want)
+        rmean, rrstd, ry, by = ref.layernorm(want, ww, bb, 1e-5)
+        bmean, brstd = ref.stats_bounds(want, rrstd)
+        ref.close(mean, rmean, bmean)
+        ref.close(rstd, rrstd, rrstd * brstd)
+        ref.close(y, ry, by)
+        del want, ry, by
+    q, scale = ref.save8(x)
+    dx, dw, db = torch.empty_like(x), torch.empty(cols, dtype=wt, device="cuda"), torch.empty(cols, dtype=wt, device="cuda")
+    for xv, kw in ((x, {"x": x.data_ptr()}), (ref.restore8(q, scale), {"q": q.data_ptr(), "scale": scale.data_ptr()})):
+        for o in (dx, dw, db):
+            o.fill_(7.0)
+        go(emac.layernorm_grad_init(rows, cols, CODE[dt], [dy.data_ptr()], mean.data_ptr(), rstd.data_ptr(), weight=w.data_ptr(), wdtype=CODE[wt],
+                                    dsum=dsum.data_ptr(), dx=dx.data_ptr(), dweight=dw.data_ptr(), dbias=db.data_ptr(), gdtype=CODE[wt], **kw))
+        rdx, bdx, rdw, bdw, rdb, bdb = ref.layernorm_grad(dy, xv, mean, rstd, w, dsum, exh=3 * ref.U)
+        ref.close(dx, rdx, bdx)
+        ref.close(dw, rdw, bdw)
+        ref.close(db, rdb, bdb)
+        del rdx, bdx, rdw, bdw, rdb, bdb
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,cols", [(3, 5), (40, 300), (700, 300), (600, 4100), (20, 20000), (300, 20000)])
+def test_added_to_in_16_bits(rows, cols, t):
+    """accumulate with gradients in 16 bits: what was there and the sum are added in 32 bits and rounded once."""
+    dt, gen = ref.TYPES[t], rnd(rows)
+    x, dy = (torch.randn(rows, cols, device="cuda", generator=gen).to(dt) for _ in range(2))
+    mean, rstd = x.float().mean(1), (x.float().var(1, unbiased=False) + 1e-5).rsqrt()
+    dw0, db0 = ((torch.randn(cols, device="cuda", generator=gen) * 20).to(dt) for _ in range(2))
+    dw, db = dw0.clone(), db0.clone()
+    go(emac.layernorm_grad_init(rows, cols, CODE[dt], [dy.data_ptr()], mean.data_ptr(), rstd.data_ptr(), x=x.data_ptr(), dweight=dw.data_ptr(),
+                                dbias=db.data_ptr(), accumulate=True))
+    _, _, rdw, bdw, rdb, bdb = ref.layernorm_grad(dy, x, mean, rstd, None, None, exh=3 * ref.U)
+    for got, was, r, bound in ((dw, dw0, rdw, bdw), (db, db0, rdb, bdb)):
+        ref.close(got, was.double() + r, bound + ref.U * (was.double().abs() + r.abs() + bound))
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_act_at_its_ends_in_16_bits(kind, t):
+    """Far tails and the largest values: the definition where it is in reach of the type, a itself far above zero, zero
+    far below it, a slope of 1 and of 0 there."""
+    dt = ref.TYPES[t]
+    top = float(torch.finfo(dt).max)
+    a = torch.tensor([[0.0, -0.0, 1e-4, -1e-4, 3.0, -3.0, 9.0, -9.0, 14.0, -14.0, 40.0, -40.0, 100.0, -100.0, 1e4, -1e4, top, -top]], device="cuda").to(dt)
+    n = a.shape[1]
+    h, da, dh = torch.empty_like(a), torch.empty_like(a), torch.ones_like(a)
+    go(emac.act_init(1, n, CODE[dt], KINDS[kind], a.data_ptr(), h.data_ptr()))
+    v, _, bv, _ = ref.act(kind, a[:, :12])
+    ref.close(h[:, :12], v, bv)
+    assert torch.equal(h[0, 12::2], a[0, 12::2]) and bool((h[0, 13::2] == 0).all())
+    back = torch.empty(1, n, device="cuda")
+    for j in range(n):  # each value a block of its own
+        one = a[:, j:j + 1].float()
+        q, s = ref.save8(one)
+        back[:, j:j + 1] = ref.restore8(q, s)
+        go(emac.act_grad_init(1, 1, CODE[dt], KINDS[kind], dh[:, j:].data_ptr(), q.data_ptr(), s.data_ptr(), da[:, j:].data_ptr()))
+    _, slope, _, bslope = ref.act(kind, back[:, :12])
+    ref.close(da[:, :12], slope, bslope + 4 * ref.U * slope.abs())
+    assert bool((da[0, 12::2] == 1).all()) and bool((da[0, 13::2] == 0).all())
