@@ -60,7 +60,7 @@ int emac_gpu_layernorm(const ext_mpi_amd_layernorm *d, void *stream) {
 
 size_t emac_gpu_layernorm_grad_ws(const ext_mpi_amd_layernorm_grad *d) {
   const grad_shape s = grad_shape_of(*d);
-  if (s.apart || s.parts <= 1 || !(d->dweight || d->dbias)) return 0;
+  if (s.apart || !(d->dweight || d->dbias)) return 0;
   return sizeof(float) * 2 * (size_t)d->cols * (size_t)s.parts;
 }
 
@@ -86,7 +86,7 @@ int emac_gpu_layernorm_grad(const ext_mpi_amd_layernorm_grad *d, float *part, vo
       default: rc = EMAC_ERR_UNSUPPORTED;
       }
     }
-    if (rc || !part) return rc; // no workspace: no column sums, or one workgroup wrote them
+    if (rc || !part) return rc; // no workspace: no column sums, or the apart form wrote them
   }
   if (!sums) return 0;
   // no rows: the sums are zeros

@@ -318,22 +318,12 @@ __device__ inline void put_grad(void *out, int gdtype, int accumulate, long c, f
   }
 }
 
-// Column sums that a workgroup has finished, 8 of each, into its partial row, or (no partial rows)
-// into the gradients
+// Column sums that a workgroup has finished, 8 of each, into its partial row
 template <int TAIL>
-__device__ inline void put_cols(const ext_mpi_amd_layernorm_grad &d, float *part, int slice, const slot<TAIL> &at, f8 w, f8 b) {
-  if (part) {
-    float *p = part + (long)slice * 2 * d.cols;
-    at.template store<float, true>(p, round_to<float>(w));
-    at.template store<float, true>(p + d.cols, round_to<float>(b));
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; j++)
-    if (at.mine(j)) {
-      if (d.dweight) put_grad(d.dweight, d.gdtype, d.accumulate, at.c + j, w[j]);
-      if (d.dbias) put_grad(d.dbias, d.gdtype, d.accumulate, at.c + j, b[j]);
-    }
+__device__ inline void put_cols(float *part, int slice, long cols, const slot<TAIL> &at, f8 w, f8 b) {
+  float *p = part + (long)slice * 2 * cols;
+  at.template store<float, true>(p, round_to<float>(w));
+  at.template store<float, true>(p + cols, round_to<float>(b));
 }
 
 // x of a row, or its checkpoint, as loaded
@@ -443,7 +433,7 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
     }
   }
   if constexpr (ACC) {
-    if (!d.dweight && !d.dbias) return;
+    if (!part) return; // no column sums are asked for
     if constexpr (!lanes<MODE>::kOneRow) { // the rows of a workgroup taken side by side, added in order
       __shared__ f8 comb[2][MODE * NV];
       for (int k = 1; k < ln.kRows; k++) {
@@ -467,7 +457,7 @@ __device__ inline void grad_rows(const ext_mpi_amd_layernorm_grad &d, int block,
       if (ln.sub) return;
     }
 #pragma unroll
-    for (int i = 0; i < NV; i++) put_cols(d, part, block, slot<TAIL>(i, per, l, cols, true), aw[i], ab[i]);
+    for (int i = 0; i < NV; i++) put_cols(part, block, d.cols, slot<TAIL>(i, per, l, cols, true), aw[i], ab[i]);
   }
 }
 
@@ -482,7 +472,8 @@ template <int LANES>
 using lanes_sums = float[512 / LANES][8 * LANES];
 
 // The column sums alone: a workgroup takes 8 * LANES columns of every slices'th group of rows, as
-// many rows at a time as it has lanes for. `part` as in put_cols.
+// many rows at a time as it has lanes for. They go into its slice's partial row, or (no partial rows) into
+// the gradients.
 template <class T, int LANES, bool Q8, bool MULTI, int TAIL>
 __device__ inline void cols_tile(const ext_mpi_amd_layernorm_grad &d, int tile, int slice, int slices, float *part,
                                  lanes_sums<LANES> *comb) {
