@@ -634,12 +634,15 @@ int norm_go(const ext_mpi_amd_layernorm &d, const row_shape &s, hipStream_t st) 
 
 // Rows of 16 to 32 KB from one leaf: a workgroup of up to 16 waves with 32 bytes of the row to a lane,
 // where row_shape_of gives fewer waves more of it (float, 8192 x 5120 with residual, sum and checkpoint
-// 131 us against 168, 4096 x 8192 112 against 129; bf16 without 4096 x 10240 36.7 against 40.2).
-// Shorter rows are slower with more waves (bf16 4096 x 8192 38.3 against 25.1), and longer ones do not
-// fit the registers (float 4096 x 12288 90 against 79).
-template <class T, int NV>
+// 131 us against 168, 4096 x 8192 112 against 129; bf16 with float weights 4096 x 8200 27.5 against 35.8,
+// 4096 x 10240 37.0 against 40.2, 4096 x 16384 49.4 against 50.1). Not in 16 bits with weights of the rows'
+// type, or none: that kernel's widened rows and weights take more than the 128 registers, and it spills (bf16
+// 4096 x 8200 118 us against 36.5, 4096 x 16384 227 against 49). Shorter rows are slower with more waves
+// (bf16 4096 x 8192 38.3 against 25.1), and longer ones do not fit the registers (float 4096 x 12288 90
+// against 79).
+template <class T, class W, int NV>
 constexpr bool sixteen() {
-  return sizeof(T) == 4 ? NV == 2 : NV == 3 || NV == 4;
+  return sizeof(T) == 4 ? NV == 2 : sizeof(W) == 4 && (NV == 3 || NV == 4);
 }
 inline int sixteen_block(long cols, int esize) { return (int)((cols * esize + 31) / 32 + 63) / 64 * 64; }
 
@@ -647,7 +650,7 @@ template <class T, class W, int MODE, int NV>
 int norm_nv(const ext_mpi_amd_layernorm &d, const row_shape &s, hipStream_t st) {
   if (tail_of(d.cols, d.q) == SHIFT) return norm_go<T, W, MODE, NV, true, SHIFT>(d, s, st);
   if (d.nsrc > 1) return norm_go<T, W, MODE, NV, true, WHOLE>(d, s, st);
-  if constexpr (sixteen<T, NV>()) {
+  if constexpr (sixteen<T, W, NV>()) {
     const int block = sixteen_block(d.cols, sizeof(T));
     return norm_go<T, W, 1024, 4 / sizeof(T), false, WHOLE>(d, row_shape{1024, 4 / (int)sizeof(T), block}, st);
   } else {
