@@ -97,6 +97,10 @@ class ExtMpiError(RuntimeError):
         self.code = code
 
 
+class ExtMpiTypeError(ExtMpiError, ValueError):
+    """An element type that an entry point of the Allreduce does not take (a ValueError, as dtype_code's own)."""
+
+
 def build(with_mpi=True):
     """Compile the native libraries in-tree (hipcc --offload-arch=gfx950)."""
     targets = ["all"] if with_mpi else [os.path.join("..", "libext_mpi_amd.so")]
@@ -181,13 +185,20 @@ def lib():
 
 
 def dtype_code(dt):
-    """Map a torch/numpy dtype (or its name) to the library's element type code."""
+    """Map a torch/numpy dtype (or its name) to the library's element type code. BF16 and HALF are taken by the row
+    operators alone: the Allreduce's and the fold's entry points raise a ValueError for them."""
     key = str(dt)
     if key in _TORCH_DTYPE_CODES:
         return _TORCH_DTYPE_CODES[key]
     if key in _NUMPY_DTYPE_CODES:
         return _NUMPY_DTYPE_CODES[key]
     raise ValueError(f"unsupported element type {dt} (float, double, int, long; bfloat16 and half for the row operators)")
+
+
+def _fold_type(what, dtype):
+    """The Allreduce and the fold add no bfloat16 and no half."""
+    if dtype in (BF16, HALF):
+        raise ExtMpiTypeError(f"{what} of bfloat16 or half", ERROR_ARG)
 
 
 def _check(what, rc):
@@ -203,6 +214,7 @@ def _enc(copyin):
 def node_allreduce_init(sendptrs, recvptrs, count, dtype, copyin=None, op=SUM):
     """Persistent Allreduce over len(sendptrs) node ranks whose buffers all live in this
     process (device or host addresses). Returns an integer handle."""
+    _fold_type("ext_mpi_amd_node_allreduce_init", dtype)
     n = len(sendptrs)
     s = (ctypes.c_void_p * n)(*sendptrs)
     r = (ctypes.c_void_p * n)(*recvptrs)
@@ -217,6 +229,7 @@ def node_comm_allreduce_init(sendptrs, recvptrs, count, dtype, comm, copyin=None
     (len(sendptrs) node ranks, device buffers on this process's GPU) and `comm` having one member
     per node (RCCL or loopback): the NODE form's copy-in, the inter-node legs of every node rank,
     the node's copy-out. Bits equal allreduce_init over size * len(sendptrs) ranks."""
+    _fold_type("ext_mpi_amd_node_comm_allreduce_init", dtype)
     n = len(sendptrs)
     s = (ctypes.c_void_p * n)(*sendptrs)
     r = (ctypes.c_void_p * n)(*recvptrs)
@@ -228,6 +241,7 @@ def node_comm_allreduce_init(sendptrs, recvptrs, count, dtype, comm, copyin=None
 
 def fold_init(srcptrs, dstptrs, count, dtype, op=SUM):
     """Persistent fold of one chunk: every dst = ((src0 + src1) + src2) + ... (device pointers)."""
+    _fold_type("ext_mpi_amd_fold_init", dtype)
     s = (ctypes.c_void_p * len(srcptrs))(*srcptrs)
     d = (ctypes.c_void_p * len(dstptrs))(*dstptrs)
     h = ctypes.c_int(-1)
@@ -365,6 +379,7 @@ def comm_free(comm):
 
 def allreduce_init(sendptr, recvptr, count, dtype, comm, copyin=None, op=SUM):
     """Persistent Allreduce of this rank's buffer over a communicator (one rank per GPU)."""
+    _fold_type("ext_mpi_amd_allreduce_init", dtype)
     h = ctypes.c_int(-1)
     _check("ext_mpi_amd_allreduce_init",
            lib().ext_mpi_amd_allreduce_init(sendptr, recvptr, count, dtype, op, comm, _enc(copyin), ctypes.byref(h)))
@@ -402,6 +417,7 @@ def node_shares(nodes, ports, ranks_per_node, count, dtype, copyin, me, max_shar
     """The parts of node rank `me`'s chunk the peer-mapped node join folds: (levels, list of
     (off, len, folding node, [leaf nodes in fold order])) -- levels 1: a left fold of the leaves,
     k: k levels of pairs of consecutive leaves (ext_mpi_amd_node_shares)."""
+    _fold_type("ext_mpi_amd_node_shares", dtype)
     off = (ctypes.c_long * max_shares)()
     ln = (ctypes.c_long * max_shares)()
     nd = (ctypes.c_int * max_shares)()
@@ -525,6 +541,7 @@ def plan_describe(nranks, count, dtype, copyin, pos, max_pieces=4096):
 
     Returns dict(owner, pieces=[(off, len)], leaves=[node ranks in fold order],
     first=[...], close=[...], nlev)."""
+    _fold_type("ext_mpi_amd_plan_describe", dtype)
     off = (ctypes.c_long * max_pieces)()
     ln = (ctypes.c_long * max_pieces)()
     owner = ctypes.c_int()
@@ -560,6 +577,7 @@ def comm_program_nodes(nodes, ranks_per_node, rank, count, dtype, copyin=None, s
     per step, 2^k nodes); ``rank`` is global (node-major). Folds are (offset, count,
     [(buf, leaf_offset)], leg) with leg LEG_FOLD (the node's fold) or LEG_NODES_FOLD | step << 8
     (the kept lines' partials in the reference's accumulator order)."""
+    _fold_type("ext_mpi_amd_comm_program_node_ports", dtype)
     ops = (P2P * max_ops)()
     folds = (FoldDesc * max_folds)()
     nops, nf, stage = ctypes.c_int(), ctypes.c_int(), ctypes.c_long()

@@ -182,3 +182,14 @@ def test_the_normal_tail():
     b = a.float()
     want = torch.special.erfcx(b.double() / math.sqrt(2)) / 2
     assert float((tail(1 / (1 + at * b)).double() / want - 1).abs().max()) < 25.1 * ref.U
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_a_fold_of_16_bits_is_a_value_error(dt):
+    """The call with the code of bfloat16 or half raises what is a ValueError and an ExtMpiError."""
+    for f in (lambda t: emac.fold_init([64], [64], 8, t), lambda t: emac.node_allreduce_init([64], [64], 8, t),
+              lambda t: emac.allreduce_init(64, 64, 8, t, 0), lambda t: emac.node_comm_allreduce_init([64], [64], 8, t, 0),
+              lambda t: emac.plan_describe(2, 64, t, "6;1 -2 2", 0), lambda t: emac.comm_program(2, 0, 64, t)):
+        with pytest.raises(ValueError):
+            f(emac.dtype_code(dt))
+        assert code_of(f, emac.dtype_code(dt)) == ARG
